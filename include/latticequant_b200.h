@@ -49,6 +49,7 @@ extern "C" {
 #define LQ_EF_NONFINITE 0x10u /* non-finite input or scaled input */
 #define LQ_EF_NOCONVERGE 0x20u /* table normalisation did not converge */
 #define LQ_EF_TIMEOUT 0x40u    /* a bulk copy into shared memory did not complete within a second */
+#define LQ_EF_PAGE 0x80u       /* a slot, page, length or draft index outside the pool or its table */
 
 /* ---- dtypes ---- */
 #define LQ_F32 0
@@ -430,6 +431,120 @@ int lq_rans_encode_streams(const int32_t *sym_idx, const int64_t *sym_off, const
                            uint32_t *state, uint32_t *err, void *stream);
 int lq_rans_finish_streams(const uint32_t *slots, const int64_t *slot_off, const int64_t *nbits, int64_t n_streams,
                            const int64_t *dst_off, uint32_t *dst, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Paged E8 cache.  The chunk layouts above hold a batch of one length; a
+ * pool of fixed-rate pages holds sequences of any length that share, fork and
+ * free their pages.  No counterpart in the reference, whose cache grows one
+ * buffer per layer by torch.cat (llm/compressed_kv_cache.py:377-395).
+ *   codes    u32 [layers][n_pages][2][n_heads][P][head_dim / 8], 16-byte
+ *            aligned (index 0 of the pair: K, 1: V); P = page_tokens, a power of two in
+ *            16..256, head_dim 64 or 128.  A word is one E8 block as the 4-bit
+ *            code of core/compact_storage.py:87-222 read as a big-endian
+ *            integer: [coset | u0..u6 (4 bits) | u7 >> 1 (3)]
+ *   scales   fp32 [layers][n_pages][2][n_heads][P], positive: one per token,
+ *            head and side; value = (u - 8 + coset/2) * scale
+ *   table    int32 [rows][width] page of tokens [P*c, P*(c+1)), -1: none;
+ *            width at most 2^20.  The layers share the tables
+ *   lens     int32 [rows] tokens held
+ *   refs     int32 [n_pages] table entries that name the page; 0: free
+ * A slot is page * P + row.  err gets LQ_EF_PAGE for indices outside the pool
+ * (the access is skipped) and may be NULL.
+ * ---------------------------------------------------------------------- */
+
+/* Quantise n_tokens tokens of one layer into their slots.  A vector (one
+ * token's K or V of one head) gets the smallest scale that keeps its points in
+ * the 4-bit range, s = amax / (7 - 1/64) (1 where amax < 1e-6), and the E8
+ * points of x / s as lq_encode_e8 finds them.  A vector with a NaN or an
+ * infinity is stored as zeros and raises LQ_EF_NONFINITE.
+ *   k, v     element (n, h, d) at n * stride_n + h * stride_h + d; 16-byte
+ *            aligned, strides multiples of 8 elements
+ *   slots    int64 [n_tokens], distinct; negative: not stored
+ *   codes, scales   one layer of the pool
+ *   k_out, v_out    optional [n_tokens][n_heads][head_dim] in dtype: the
+ *            stored values (point * scale), 16-byte aligned */
+int lq_paged_append(const void *k, const void *v, int dtype, int64_t n_tokens, int n_heads, int head_dim,
+                    int64_t k_stride_n, int64_t k_stride_h, int64_t v_stride_n, int64_t v_stride_h,
+                    const int64_t *slots, int64_t n_pages, int page_tokens, int32_t *codes, float *scales,
+                    void *k_out, void *v_out, uint32_t *err, void *stream);
+
+/* Attention of n_query positions a sequence over its pages: position t reads
+ * the tokens before the last n_query (the context) and, of those last ones
+ * (the drafts, position t's own among them), draft j where mask[t][j] != 0,
+ * or j <= t without a mask.  One position without a mask is a decode step.
+ *   q        [batch][n_heads * group][n_query][head_dim], LQ_F16 or LQ_BF16,
+ *            16-byte aligned, strides (elements) multiples of 8; query head
+ *            h * group + g reads KV head h
+ *   lens     tokens in the pages, the drafts included; max_len bounds them
+ *            (longer ones are cut, with LQ_EF_PAGE)
+ *   mask     bytes [n_query][n_query], sequences mask_stride_b apart (0: one
+ *            for all); NULL: causal
+ *   out      [batch][n_heads * group][n_query][head_dim] in q's type
+ *   lse      optional fp32 [batch][n_heads * group][n_query], natural log.  A
+ *            position that sees no token gets o = 0, lse = -inf
+ * n_query 1..4096, group 1..64. */
+size_t lq_paged_attention_workspace(int64_t batch, int n_heads, int group, int64_t n_query, int head_dim,
+                                    int64_t max_len);
+int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+                       const int32_t *codes, const float *scales, int64_t n_pages, int page_tokens,
+                       const int32_t *table, int64_t table_width, int64_t table_stride, const int32_t *lens,
+                       int64_t max_len, const uint8_t *mask, int64_t mask_stride_b, int64_t batch, int n_heads,
+                       int group, int64_t n_query, int head_dim, float sm_scale, void *out, float *lse,
+                       void *workspace, size_t workspace_bytes, uint32_t *err, void *stream);
+
+/* Fork, free and reserve: new tables whose row i continues row parents[i] of
+ * the old ones (-1: an empty row; rows named by no child are freed), with
+ * pages for `reserve` more tokens.  Full pages are shared.  The page a row
+ * writes to next, and reserved ones, stay with the row's first child; other
+ * children get fresh pages, the lowest free ones in order of child and
+ * column, with the live rows copied in all layers.  Entries past the reserve
+ * are -1.  Out of place: outputs alias no input.  Too few free pages leave
+ * -1 entries and raise LQ_EF_CAPACITY. */
+size_t lq_pages_fork_workspace(int64_t rows, int64_t children, int64_t n_pages);
+int lq_pages_fork(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens, const int32_t *refs,
+                  const int64_t *parents, int64_t children, int64_t reserve, int32_t *new_table, int32_t *new_lens,
+                  int32_t *new_refs, int32_t *codes, float *scales, int64_t n_layers, int64_t n_pages, int n_heads,
+                  int page_tokens, int head_dim, void *workspace, size_t workspace_bytes, uint32_t *err, void *stream);
+
+/* Move the live pages to the front of the pool: with n_live pages in use, those
+ * at or above n_live go, in order, to the free ones below it, in all layers.
+ *   table    [entries] old pages (any number of rows), new_table the new ones
+ *   n_live   one int32 on the device.  Outputs alias no input. */
+size_t lq_pages_compact_workspace(int64_t n_pages);
+int lq_pages_compact(const int32_t *table, int64_t entries, const int32_t *refs, int32_t *new_table,
+                     int32_t *new_refs, int32_t *n_live, int32_t *codes, float *scales, int64_t n_layers,
+                     int64_t n_pages, int n_heads, int page_tokens, int head_dim, void *workspace,
+                     size_t workspace_bytes, uint32_t *err, void *stream);
+
+/* Copy pages src[i] to dst[i], i < *count (on the device, at most `most`), in
+ * all layers; no dst is a src and no dst is named twice. */
+int lq_pages_copy(const int32_t *src, const int32_t *dst, const int32_t *count, int64_t most, int32_t *codes,
+                  float *scales, int64_t n_layers, int64_t n_pages, int n_heads, int page_tokens, int head_dim,
+                  uint32_t *err, void *stream);
+
+/* Keep the accepted drafts: the last n_draft tokens of every row are drafts;
+ * accepted[b][0..] names the ones to keep, strictly ascending, ended by a
+ * negative entry or by `most`.  Their rows move to the front of the drafts'
+ * slots in all layers; new_lens (not lens itself) = lens - n_draft + kept.
+ * A row whose list is not ascending or out of range is left as it is. */
+int lq_pages_accept(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens, int64_t n_draft,
+                    const int32_t *accepted, int64_t most, int32_t *new_lens, int32_t *codes, float *scales,
+                    int64_t n_layers, int64_t n_pages, int n_heads, int page_tokens, int head_dim, uint32_t *err,
+                    void *stream);
+
+/* ------------------------------------------------------------------------
+ * Beam search's selection: the n largest of scores[b][k] + ln softmax(x[b][k])[v]
+ * over the beams k and words v of each sequence b, best first; equal totals go
+ * to the lower beam, then the larger logit, then the lower word.  Words with a
+ * logit of -inf or NaN, beams with a score of -inf or NaN or a logit of +inf
+ * give no candidate; places left over hold -inf, -1, -1.
+ *   logits   element (b, k, v) at b * stride_b + k * stride_k + v, any strides
+ *   n 1..128, beams 1..256, vocab up to 2^24, batch * beams up to 65535.
+ * ---------------------------------------------------------------------- */
+size_t lq_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t n);
+int lq_beam_select(const void *logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t stride_b,
+                   int64_t stride_k, const float *scores, int64_t n, float *top_score, int64_t *top_beam,
+                   int64_t *top_word, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------
  * Diagnostics for tests: run one internal device helper over arrays.

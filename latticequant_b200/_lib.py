@@ -20,6 +20,7 @@ LQ_OK = 0
 LQ_ERR_INVALID, LQ_ERR_ALPHABET, LQ_ERR_CAPACITY, LQ_ERR_CUDA, LQ_ERR_STREAM = -1, -2, -3, -4, -5
 EF_ALPHABET, EF_SYMRANGE, EF_CAPACITY, EF_BITSTREAM, EF_NONFINITE, EF_NOCONVERGE = 0x1, 0x2, 0x4, 0x8, 0x10, 0x20
 EF_TIMEOUT = 0x40
+EF_PAGE = 0x80
 LQ_F32, LQ_F16, LQ_BF16 = 0, 1, 2
 L = 1024
 SYM_LIMIT = 512
@@ -35,6 +36,7 @@ _FLAG_TEXT = {
     EF_NONFINITE: "non-finite value in the input or in input/scale",
     EF_NOCONVERGE: "rANS frequency normalisation did not converge",
     EF_TIMEOUT: "a bulk copy into shared memory did not complete within a second",
+    EF_PAGE: "a slot, page, length or draft index lies outside the page pool or its table",
 }
 
 _lib = None
@@ -113,6 +115,19 @@ def _declare(lib):
         "lq_unpack_bits": ([vp, i64, vp, vp], i32),
         "lq_map_symbols": ([vp, i64, vp, ctypes.c_int32, i32, vp, vp], i32),
         "lq_rans_encode_streams": ([vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp], i32),
+        "lq_paged_append": ([vp, vp, i32, i64, i32, i32, i64, i64, i64, i64, vp, i64, i32, vp, vp, vp, vp, vp, vp], i32),
+        "lq_paged_attention_workspace": ([i64, i32, i32, i64, i32, i64], sz),
+        "lq_paged_attention": ([vp, i32, i64, i64, i64, vp, vp, i64, i32, vp, i64, i64, vp, i64, vp, i64, i64, i32, i32,
+                                i64, i32, f32, vp, vp, vp, sz, vp, vp], i32),
+        "lq_pages_fork_workspace": ([i64, i64, i64], sz),
+        "lq_pages_fork": ([vp, i64, i64, vp, vp, vp, i64, i64, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, vp, sz, vp,
+                           vp], i32),
+        "lq_pages_compact_workspace": ([i64], sz),
+        "lq_pages_compact": ([vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, vp, sz, vp, vp], i32),
+        "lq_pages_copy": ([vp, vp, vp, i64, vp, vp, i64, i64, i32, i32, i32, vp, vp], i32),
+        "lq_pages_accept": ([vp, i64, i64, vp, i64, vp, i64, vp, vp, vp, i64, i64, i32, i32, i32, vp, vp], i32),
+        "lq_beam_select_workspace": ([i64, i64, i64, i64], sz),
+        "lq_beam_select": ([vp, i32, i64, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, sz, vp], i32),
         "lq_rans_finish_streams": ([vp, vp, vp, i64, vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():

@@ -1,0 +1,468 @@
+// lq_paged_attn.cu -- attention of a block of query positions over the pages
+// of an E8 cache, on warp-level tensor-core instructions.
+//
+// For every sequence b, query head hq = h * G + g and position t < T:
+//   o = softmax(q . K^T * sm_scale) V  over the tokens p < len[b] that t sees:
+//   all of the context (p < len - T) and, of the last T tokens (the drafts),
+//   those whose mask[t][p - (len - T)] is set (without a mask: drafts <= t).
+// The reference has no counterpart: its decode attends one position over the
+// dequantised buffer (llm/compressed_kv_cache.py:342-395).
+//
+// Mathematics.  A query row r = t * G + g; the tile of a warp is 16 tokens by
+// 8 * NT rows.  Scores S = K Q^T put tokens on the rows of the MMA, so a
+// lane's A registers are whole code words of "its" two tokens, decoded in
+// registers: values are exact in q's own type (fp16 or bf16) and the token's
+// scale multiplies the fp32 score.  V's scale goes into the exponent:
+//   x = s * log2(e) * sm_scale * ks + log2(vs),  w = 2^(x - M),
+//   o += w * point,  l += w / vs
+// so the fp16 weights w stay within 2^14 whatever the scales are.  M is a
+// reference, not the running maximum: it moves (to the maximum less 6) only
+// when an x exceeds it by 14, which a warp vote finds; the statistics are
+// then rescaled.  W^T reaches its B registers with one 8x8 transpose per 8
+// tokens; V's A registers pair two tokens' decoded channels by byte permutes.
+#include "lq_paged.cuh"
+#include "lq_paged_attn.cuh"
+
+namespace lq {
+namespace {
+
+constexpr int kWarps = 4;
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    if constexpr (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint32_t *p, uint32_t w[N]) {
+    if constexpr (N == 4) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = u.x;
+        w[1] = u.y;
+        w[2] = u.z;
+        w[3] = u.w;
+    } else if constexpr (N == 2) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = u.x;
+        w[1] = u.y;
+    } else {
+        w[0] = __ldg(p);
+    }
+}
+
+// What a lane (g = lane / 4, t = lane % 4) reads of a 16-token tile: K words
+// t*KW.. of tokens g and g + 8, V words g*VW.. of tokens 2t, 2t+1, 2t+8,
+// 2t+9, and the scales of tokens g and g + 8.
+template <int D>
+struct Tile {
+    static constexpr int KW = D / 32, VW = D / 64;
+    uint32_t k[2][KW], v[4][VW];
+    float ks[2], vs[2];
+};
+
+template <int D>
+__device__ __forceinline__ void load_tile(const PagedAttnArgs &a, const uint32_t *kbase, const float *sbase, int64_t page,
+                                          uint32_t off, uint32_t g, uint32_t t, Tile<D> &x) {
+    constexpr int W = D / 8;
+    // the page's K rows of this head (kbase is the head's offset in page 0)
+    const int64_t side = (int64_t)a.n_heads << a.page_log2;
+    const int64_t row = 2 * side * page + off;
+    const uint32_t *kp = kbase + row * W;
+    const uint32_t *vp = kp + side * W;
+    const float *sp = sbase + row;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        load_words<Tile<D>::KW>(kp + (g + 8 * r) * W + t * Tile<D>::KW, x.k[r]);
+        x.ks[r] = __ldg(sp + g + 8 * r);
+        x.vs[r] = __ldg(sp + side + g + 8 * r);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        load_words<Tile<D>::VW>(vp + (2 * t + (i & 1) + 8 * (i >> 1)) * W + g * Tile<D>::VW, x.v[i]);
+}
+
+// Both 16-bit halves of two registers, regrouped: lo = (a.lo, b.lo), hi = (a.hi, b.hi).
+__device__ __forceinline__ void zip_halves(uint32_t a, uint32_t b, uint32_t &lo, uint32_t &hi) {
+    lo = __byte_perm(a, b, 0x5410);
+    hi = __byte_perm(a, b, 0x7632);
+}
+
+template <int D, int NT, int S>
+__device__ __forceinline__ void pv_step(const CodeWord c[4][D / 64], const uint32_t (*p)[2], float (*o)[NT][4]) {
+    if constexpr (D == 128) {
+        uint32_t a[4], b[4];  // [block * 2 + token group] for the pair's two channels
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                zip_halves(code_pair<false, S>(c[2 * half][blk]), code_pair<false, S>(c[2 * half + 1][blk]),
+                           a[blk + 2 * half], b[blk + 2 * half]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            mma_16816<false>(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
+            mma_16816<false>(o[4 + S][n], b[0], b[1], b[2], b[3], p[n][0], p[n][1]);
+        }
+    } else {
+        uint32_t a[4];  // one block: its two channels are the MMA's two row groups
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+            zip_halves(code_pair<false, S>(c[2 * half][0]), code_pair<false, S>(c[2 * half + 1][0]), a[2 * half],
+                       a[1 + 2 * half]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_16816<false>(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
+    }
+}
+
+// grid (splits, n_heads * row tiles, batch); a CTA's warps take the 16-token
+// tiles of its chunk in turn.
+template <bool BF16, int D, int NT>
+__global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int KW = D / 32, VW = D / 64, W = D / 8, MT = D / 16;
+    constexpr int ROWS = 8 * NT;
+    extern __shared__ __align__(16) float sm[];  // [warps][ROWS][D + 2]
+    const int warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t b = blockIdx.z, rt = blockIdx.y / a.n_heads, h = blockIdx.y - rt * a.n_heads;
+    const uint32_t row0 = rt * ROWS;
+    const int64_t len = paged_len(a, b);
+    const int64_t first = (int64_t)blockIdx.x * a.chunk, last = min(first + a.chunk, len);
+    const int64_t drafts = len - a.T;  // position of draft 0
+    if (len < a.lens[b] && (blockIdx.x | blockIdx.y | threadIdx.x) == 0) raise_flag(a.err, LQ_EF_PAGE);
+
+    // Q's B registers: row n = lane / 4 of each 8-row group, this lane's blocks
+    uint32_t qf[NT][KW * 4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const uint32_t r = row0 + 8 * n + g;
+        const bool in = r < a.rows;
+        const uint32_t qt = in ? a.by_group.div(r) : 0, qh = h * a.group + (in ? r - qt * a.group : 0);
+        const uint4 *qp = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
+                                                          qh * a.q_stride_h + qt * a.q_stride_t);
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (in) u = __ldg(qp + t * KW + j);
+            // code_pair S holds channels (7 - S, 3 - S): low half channel 7 - S
+            qf[n][4 * j + 0] = __byte_perm(u.w, u.y, 0x7632);
+            qf[n][4 * j + 1] = __byte_perm(u.w, u.y, 0x5410);
+            qf[n][4 * j + 2] = __byte_perm(u.z, u.x, 0x7632);
+            qf[n][4 * j + 3] = __byte_perm(u.z, u.x, 0x5410);
+        }
+    }
+
+    float o[MT][NT][4], l[NT][2], m[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[i][n][c] = 0.f;
+        l[n][0] = l[n][1] = 0.f;
+        m[n][0] = m[n][1] = kNoRef;
+    }
+
+    const int32_t *table = a.table + b * a.table_stride;
+    const uint32_t *kbase = a.codes + ((int64_t)h << a.page_log2) * W;
+    const float *sbase = a.scales + ((int64_t)h << a.page_log2);
+    const uint32_t page_mask = (1u << a.page_log2) - 1;
+    // a table entry outside the pool is reported, and read as page 0 with its tokens masked
+    auto page_of = [&](int64_t tok) -> int64_t {
+        return tok < last ? (int64_t)__ldg(table + (tok >> a.page_log2)) : 0;
+    };
+    auto usable = [&](int64_t page) { return page >= 0 && page < a.n_pages; };
+
+    int64_t tok = first + 16 * warp;
+    Tile<D> nx;
+    int64_t page_nx = page_of(tok);
+    if (tok < last) load_tile<D>(a, kbase, sbase, usable(page_nx) ? page_nx : 0, (uint32_t)tok & page_mask, g, t, nx);
+    int64_t page_nn = page_of(tok + 16 * kWarps);
+    for (; tok < last; tok += 16 * kWarps) {
+        const Tile<D> x = nx;
+        const bool bad = !usable(page_nx);
+        page_nx = page_nn;
+        const int64_t tn = tok + 16 * kWarps;
+        if (tn < last) load_tile<D>(a, kbase, sbase, usable(page_nx) ? page_nx : 0, (uint32_t)tn & page_mask, g, t, nx);
+        page_nn = page_of(tn + 16 * kWarps);
+
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            const CodeWord c0 = code_word<BF16>(x.k[0][j]), c1 = code_word<BF16>(x.k[1][j]);
+            const uint32_t a0 = code_pair<BF16, 0>(c0), a1 = code_pair<BF16, 0>(c1);
+            const uint32_t a2 = code_pair<BF16, 1>(c0), a3 = code_pair<BF16, 1>(c1);
+            const uint32_t a4 = code_pair<BF16, 2>(c0), a5 = code_pair<BF16, 2>(c1);
+            const uint32_t a6 = code_pair<BF16, 3>(c0), a7 = code_pair<BF16, 3>(c1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma_16816<BF16>(s[n], a0, a1, a2, a3, qf[n][4 * j], qf[n][4 * j + 1]);
+                mma_16816<BF16>(s[n], a4, a5, a6, a7, qf[n][4 * j + 2], qf[n][4 * j + 3]);
+            }
+        }
+
+        // x = s * ks + log2(vs), and 1 / vs for the denominator
+        float rvs[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float kx = x.ks[r] * (a.qk_log2 * kCodeUnit<BF16>), lv = __log2f(x.vs[r]);
+            rvs[r] = __frcp_rn(x.vs[r]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                s[n][2 * r] = fmaf(s[n][2 * r], kx, lv);
+                s[n][2 * r + 1] = fmaf(s[n][2 * r + 1], kx, lv);
+            }
+        }
+        if (tok + 16 > drafts || bad) {  // drafts, tokens past the end: whole warp
+            if (bad && lane == 0) raise_flag(a.err, LQ_EF_PAGE);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int64_t p = tok + g + 8 * r;
+                const bool past = p >= last || bad;
+                if (past) rvs[r] = 0.f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t row = row0 + 8 * n + 2 * t + c;
+                        if (past || (p >= drafts && row < a.rows && !paged_sees(a, b, a.by_group.div(row), p - drafts)))
+                            s[n][2 * r + c] = -INFINITY;
+                    }
+            }
+        }
+
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) grow |= fmaxf(s[n][c], s[n][2 + c]) > m[n][c] + kRefSlack;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float mx = fmaxf(s[n][c], s[n][2 + c]);
+#pragma unroll
+                    for (int off = 4; off <= 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                    const float mn = fmaxf(m[n][c], mx - kRefBelow);
+                    const float f = exp2f(m[n][c] - mn);
+                    m[n][c] = mn;
+                    l[n][c] *= f;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        o[i][n][c] *= f;
+                        o[i][n][2 + c] *= f;
+                    }
+                }
+        }
+
+        uint32_t p[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float w0 = ex2(s[n][2 * r] - m[n][0]), w1 = ex2(s[n][2 * r + 1] - m[n][1]);
+                l[n][0] = fmaf(w0, rvs[r], l[n][0]);
+                l[n][1] = fmaf(w1, rvs[r], l[n][1]);
+                const __half2 hw = __floats2half2_rn(w0, w1);
+                p[n][r] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&hw));
+            }
+
+        CodeWord c[4][VW];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < VW; ++j) c[i][j] = code_word<false>(x.v[i][j]);
+        pv_step<D, NT, 0>(c, p, o);
+        pv_step<D, NT, 1>(c, p, o);
+        pv_step<D, NT, 2>(c, p, o);
+        pv_step<D, NT, 3>(c, p, o);
+    }
+
+    // the warps' statistics and outputs, merged in warp order
+    constexpr int rs = D + 2;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int off = 4; off <= 16; off <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
+            float *dst = sm + (warp * ROWS + 8 * n + 2 * t + c) * rs;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if constexpr (D == 128) {  // tile i: channel 7 - i of blocks 2g and 2g + 1
+                    dst[16 * g + 7 - i] = o[i][n][c];
+                    dst[16 * g + 15 - i] = o[i][n][2 + c];
+                } else {  // tile i: channels 7 - i and 3 - i of block g
+                    dst[8 * g + 7 - i] = o[i][n][c];
+                    dst[8 * g + 3 - i] = o[i][n][2 + c];
+                }
+            }
+            if (g == 0) {
+                dst[D] = m[n][c];
+                dst[D + 1] = l[n][c];
+            }
+        }
+    __syncthreads();
+    const uint32_t live = min((uint32_t)ROWS, a.rows - row0);
+    for (uint32_t e = threadIdx.x; e < live * D; e += 32 * kWarps) {
+        const uint32_t r = e / D, d = e % D;
+        float mx = kNoRef;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm[(w * ROWS + r) * rs + D]);
+        float od = 0.f, ld = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float *src = sm + (w * ROWS + r) * rs;
+            const float f = ex2(src[D] - mx);
+            od = fmaf(src[d], f, od);
+            ld = fmaf(src[D + 1], f, ld);
+        }
+        paged_emit<BF16, D>(a, b, h, row0 + r, d, blockIdx.x, od, ld, mx);
+    }
+}
+
+// One row per group of D threads: the splits' partial results joined in split order.
+template <bool BF16, int D>
+__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a, uint32_t n_rows) {
+    const uint32_t i = blockIdx.x * (128 / D) + threadIdx.x / D, d = threadIdx.x % D;
+    if (i >= n_rows) return;
+    const uint32_t bh = i / a.rows, r = i - bh * a.rows;
+    const uint32_t b = bh / a.n_heads, h = bh - b * a.n_heads;
+    const float *p = a.part + ((int64_t)bh * a.splits * a.rows + r) * (D + 2);
+    const int64_t step = (int64_t)a.rows * (D + 2);
+    const int64_t len = paged_len(a, b);
+    const uint32_t used = (uint32_t)ceil_div(len, a.chunk);
+    float mx = kNoRef;
+    for (uint32_t s = 0; s < used; ++s) mx = fmaxf(mx, p[s * step + D]);
+    float od = 0.f, ld = 0.f;
+    for (uint32_t s = 0; s < used; ++s) {
+        const float f = ex2(p[s * step + D] - mx);
+        od = fmaf(p[s * step + d], f, od);
+        ld = fmaf(p[s * step + D + 1], f, ld);
+    }
+    paged_store<BF16, D>(a, b, h, r, d, od, ld, mx);
+}
+
+template <bool BF16, int D, int NT>
+int launch_rows(const PagedAttnArgs &a, uint32_t batch, cudaStream_t st) {
+    const size_t smem = (size_t)kWarps * 8 * NT * (D + 2) * 4;
+    const uint32_t tiles = (uint32_t)ceil_div(a.rows, 8 * NT);
+    paged_attn_kernel<BF16, D, NT><<<dim3(a.splits, a.n_heads * tiles, batch), 32 * kWarps, smem, st>>>(a);
+    if (check_launch() != LQ_OK) return LQ_ERR_CUDA;
+    if (a.splits > 1) {
+        const uint32_t n = batch * a.n_heads * a.rows;
+        paged_combine_kernel<BF16, D><<<(unsigned)ceil_div(n, 128 / D), 128, 0, st>>>(a, n);
+    }
+    return check_launch();
+}
+
+template <bool BF16, int D>
+int launch_dim(const PagedAttnArgs &a, uint32_t batch, cudaStream_t st) {
+    return a.rows <= 8 ? launch_rows<BF16, D, 1>(a, batch, st) : launch_rows<BF16, D, 2>(a, batch, st);
+}
+
+// Tokens of one split: enough CTAs for about four rounds of the GPU, chunks
+// of at least 64 tokens (a tile for each warp).
+struct Plan {
+    int64_t chunk;
+    uint32_t splits;
+};
+
+Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
+    const int64_t tiles = ceil_div(rows, rows <= 8 ? 8 : 16);
+    const int64_t units = batch * n_heads * tiles;  // CTAs without a split
+    const int64_t want = ceil_div((int64_t)148 * 16, units);
+    int64_t chunk = ceil_div(ceil_div(max_len < 1 ? 1 : max_len, want), 64) * 64;
+    return Plan{chunk, (uint32_t)ceil_div(max_len < 1 ? 1 : max_len, chunk)};
+}
+
+}  // namespace
+}  // namespace lq
+
+using namespace lq;
+
+static bool paged_shape_ok(int64_t batch, int n_heads, int group, int64_t n_query, int head_dim) {
+    return batch >= 0 && batch <= 65535 && n_heads >= 1 && n_heads <= 1024 && group >= 1 && group <= 64 && n_query >= 1 &&
+           n_query <= 4096 && paged_dim_ok(head_dim) && n_heads * ceil_div(n_query * group, 8) <= 65535 &&
+           batch * n_heads * n_query * group <= 0x7fffffff;
+}
+
+extern "C" size_t lq_paged_attention_workspace(int64_t batch, int n_heads, int group, int64_t n_query, int head_dim,
+                                               int64_t max_len) {
+    if (!paged_shape_ok(batch, n_heads, group, n_query, head_dim) || max_len < 0) return 0;
+    const Plan p = plan(batch, n_heads, n_query * group, max_len);
+    return p.splits > 1 ? (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 2) * 4 : 0;
+}
+
+extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+                                  const int32_t *codes, const float *scales, int64_t n_pages, int page_tokens,
+                                  const int32_t *table, int64_t table_width, int64_t table_stride, const int32_t *lens,
+                                  int64_t max_len, const uint8_t *mask, int64_t mask_stride_b, int64_t batch,
+                                  int n_heads, int group, int64_t n_query, int head_dim, float sm_scale, void *out,
+                                  float *lse, void *workspace, size_t workspace_bytes, uint32_t *err, void *stream) {
+    LQ_NVTX_RANGE();
+    if (!paged_shape_ok(batch, n_heads, group, n_query, head_dim) || !paged_page_ok(page_tokens) || n_pages < 1 ||
+        n_pages > 0x7fffffff || table_width < 0 || table_width > (1 << 20) || max_len < 0 ||
+        (q_dtype != LQ_F16 && q_dtype != LQ_BF16))
+        return LQ_ERR_INVALID;
+    if (batch == 0) return LQ_OK;
+    if (!q || !codes || !scales || (!table && table_width > 0) || !lens || !out) return LQ_ERR_INVALID;
+    const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(codes);
+    if ((al & 15) != 0 || ((q_stride_b | q_stride_h | q_stride_t) & 7) != 0) return LQ_ERR_INVALID;
+    // tokens past max_len would have no split: the caller's bound is the table's at most
+    const int64_t cap = table_width * page_tokens;
+    const int64_t bound = max_len < cap ? max_len : cap;
+    const Plan p = plan(batch, n_heads, n_query * group, bound);
+    if (p.splits > 1) {
+        if (!workspace) return LQ_ERR_INVALID;
+        if (workspace_bytes < (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 2) * 4)
+            return LQ_ERR_CAPACITY;
+    }
+    PagedAttnArgs a{};
+    a.q = q;
+    a.q_stride_b = q_stride_b;
+    a.q_stride_h = q_stride_h;
+    a.q_stride_t = q_stride_t;
+    a.codes = reinterpret_cast<const uint32_t *>(codes);
+    a.scales = scales;
+    a.n_pages = n_pages;
+    a.page_log2 = (uint32_t)__builtin_ctz((unsigned)page_tokens);
+    a.table = table;
+    a.table_width = table_width;
+    a.table_stride = table_stride;
+    a.lens = lens;
+    a.bound = bound;
+    a.mask = mask;
+    a.mask_stride_b = mask_stride_b;
+    a.n_heads = (uint32_t)n_heads;
+    a.group = (uint32_t)group;
+    a.T = (uint32_t)n_query;
+    a.rows = (uint32_t)(n_query * group);
+    a.by_group = FastDiv((uint32_t)group);
+    a.chunk = p.chunk;
+    a.splits = p.splits;
+    a.qk_log2 = sm_scale * kLog2e;
+    a.out = out;
+    a.lse = lse;
+    a.part = static_cast<float *>(workspace);
+    a.err = err;
+    cudaStream_t st = as_stream(stream);
+    const uint32_t B = (uint32_t)batch;
+    if (q_dtype == LQ_BF16) return head_dim == 128 ? launch_dim<true, 128>(a, B, st) : launch_dim<true, 64>(a, B, st);
+    return head_dim == 128 ? launch_dim<false, 128>(a, B, st) : launch_dim<false, 64>(a, B, st);
+}

@@ -1,0 +1,80 @@
+// lq_paged_attn.cuh -- arguments and epilogue shared by the attention kernels
+// over the paged E8 cache.
+#pragma once
+
+#include "lq_paged.cuh"
+
+namespace lq {
+
+struct PagedAttnArgs {
+    const void *q;  // 16-bit elements, last dimension contiguous
+    int64_t q_stride_b, q_stride_h, q_stride_t;
+    const uint32_t *codes;
+    const float *scales;
+    int64_t n_pages;
+    uint32_t page_log2;
+    const int32_t *table;  // [batch][table_width], rows table_stride apart
+    int64_t table_width, table_stride;
+    const int32_t *lens;
+    int64_t bound;        // tokens a sequence may have at most
+    const uint8_t *mask;  // [batch or 1][T][T], or NULL: drafts <= t
+    int64_t mask_stride_b;
+    uint32_t n_heads, group, T, rows;  // rows = T * group, row = t * group + g
+    FastDiv by_group;
+    int64_t chunk;  // tokens of a split
+    uint32_t splits;
+    float qk_log2;  // sm_scale * log2(e)
+    void *out;      // [batch][n_heads * group][T][D] in q's type
+    float *lse;     // [batch][n_heads * group][T] natural log, may be NULL
+    float *part;    // [batch][n_heads][splits][rows][D + 2]: o, reference, denominator
+    uint32_t *err;
+};
+
+// The reference M of the base-2 weights 2^(x - M): "none yet", how far an x
+// may exceed it (fp16 holds 2^15), and how far below the maximum it is put
+// (headroom that keeps smaller weights out of fp16's subnormals).
+constexpr float kNoRef = -1e30f, kRefSlack = 14.f, kRefBelow = 6.f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ int64_t paged_len(const PagedAttnArgs &a, uint32_t b) {
+    return min(max((int64_t)a.lens[b], (int64_t)0), a.bound);
+}
+
+// Whether position t of sequence b sees draft j.
+__device__ __forceinline__ bool paged_sees(const PagedAttnArgs &a, uint32_t b, uint32_t t, int64_t j) {
+    return a.mask ? a.mask[b * a.mask_stride_b + (int64_t)t * a.T + j] != 0 : j <= (int64_t)t;
+}
+
+// Channel d of row r from its weighted sum, denominator and reference.
+template <bool BF16, int D>
+__device__ __forceinline__ void paged_store(const PagedAttnArgs &a, uint32_t b, uint32_t h, uint32_t r, uint32_t d,
+                                            float o, float l, float m) {
+    const uint32_t t = a.by_group.div(r), qh = h * a.group + (r - t * a.group);
+    const int64_t row = ((int64_t)b * a.n_heads * a.group + qh) * a.T + t;
+    // a row that sees nothing has l = 0 (a NaN denominator stays NaN)
+    Elem<BF16 ? LQ_BF16 : LQ_F16>::store(a.out, row * D + d, l == 0.f ? 0.f : o * kCodeUnit<false> / l);
+    if (a.lse && d == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// paged_store, or the split's partial result.
+template <bool BF16, int D>
+__device__ __forceinline__ void paged_emit(const PagedAttnArgs &a, uint32_t b, uint32_t h, uint32_t r, uint32_t d,
+                                           uint32_t split, float o, float l, float m) {
+    if (a.splits == 1) {
+        paged_store<BF16, D>(a, b, h, r, d, o, l, m);
+        return;
+    }
+    float *p = a.part + (((int64_t)(b * a.n_heads + h) * a.splits + split) * a.rows + r) * (D + 2);
+    p[d] = o;
+    if (d == 0) {
+        p[D] = m;
+        p[D + 1] = l;
+    }
+}
+
+}  // namespace lq
