@@ -541,7 +541,7 @@ int lq_pages_accept(const int32_t *table, int64_t rows, int64_t width, const int
  *   logits   element (b, k, v) at b * stride_b + k * stride_k + v, any strides
  *   n 1..128, beams 1..256, vocab up to 2^24, batch * beams up to 65535.
  * ---------------------------------------------------------------------- */
-size_t lq_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t n);
+size_t lq_beam_select_workspace(int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t n);
 int lq_beam_select(const void *logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t stride_b,
                    int64_t stride_k, const float *scores, int64_t n, float *top_score, int64_t *top_beam,
                    int64_t *top_word, void *workspace, size_t workspace_bytes, void *stream);

@@ -126,7 +126,7 @@ def _declare(lib):
         "lq_pages_compact": ([vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, vp, sz, vp, vp], i32),
         "lq_pages_copy": ([vp, vp, vp, i64, vp, vp, i64, i64, i32, i32, i32, vp, vp], i32),
         "lq_pages_accept": ([vp, i64, i64, vp, i64, vp, i64, vp, vp, vp, i64, i64, i32, i32, i32, vp, vp], i32),
-        "lq_beam_select_workspace": ([i64, i64, i64, i64], sz),
+        "lq_beam_select_workspace": ([i32, i64, i64, i64, i64], sz),
         "lq_beam_select": ([vp, i32, i64, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, sz, vp], i32),
         "lq_rans_finish_streams": ([vp, vp, vp, i64, vp, vp, vp], i32),
     }
@@ -177,6 +177,20 @@ def ptr(t: torch.Tensor | None):
 
 def stream_handle(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def call(name: str, index: int, *args):
+    """The entry point `name` on device `index` and its current stream (the last
+    argument), raised as check() does.  What a call costs on the host bounds the
+    small operators, so this avoids Stream and device-guard objects."""
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != LQ_OK:
+        check(status, name)
 
 
 def check(status: int, what: str):

@@ -6,12 +6,13 @@ step's logits once and returns the best continuations; its beams are the
 """
 from __future__ import annotations
 
+import functools
 from typing import Tuple
 
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr, stream_handle
+from ._lib import call, lib
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -23,9 +24,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
     larger logit, then the lower word.  Banned words (logits of -inf, NaN) and
     dead beams (scores of -inf) are never chosen; places left without a
     candidate hold -inf, -1, -1.  n up to 128, K up to 256."""
-    _lib.require_cuda(logits)
-    if logits.dim() != 3 or scores.shape != logits.shape[:2] or scores.dtype != torch.float32 or \
-            scores.device != logits.device:
+    if not logits.is_cuda:
+        _lib.require_cuda(logits)
+    index = logits.get_device()
+    if logits.dim() != 3 or scores.shape != logits.shape[:2] or scores.dtype is not torch.float32 or \
+            scores.get_device() != index:
         raise ValueError("beam_select takes logits (B, K, V) and fp32 scores (B, K) on one device")
     B, K, V = logits.shape
     if V == 0 or K == 0 or not 1 <= n <= 128 or K > 256 or V > 1 << 24:
@@ -33,13 +36,17 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
     if logits.stride(2) != 1 and V > 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
-    dev = logits.device
-    top = torch.empty((B, n), dtype=torch.float32, device=dev)
-    beams, words = torch.empty((2, B, n), dtype=torch.int64, device=dev).unbind(0)
-    with torch.cuda.device(dev):
-        need = lib().lq_beam_select_workspace(B, K, V, n)
-        ws = torch.empty(max(need, 8), dtype=torch.uint8, device=dev)
-        check(lib().lq_beam_select(ptr(logits), _lib.dtype_code(logits.dtype), B, K, V, logits.stride(0),
-                                   logits.stride(1), ptr(scores), n, ptr(top), ptr(beams), ptr(words), ptr(ws),
-                                   ws.numel(), stream_handle(dev)), "lq_beam_select")
+    top = scores.new_empty((B, n))
+    beams = scores.new_empty((B, n), dtype=torch.int64)
+    words = torch.empty_like(beams)
+    dtype = _lib.dtype_code(logits.dtype)
+    need = _workspace(dtype, B, K, V, n)
+    ws = beams.new_empty(need // 8 + 1)
+    call("lq_beam_select", index, logits.data_ptr(), dtype, B, K, V, *logits.stride()[:2], scores.data_ptr(), n,
+         top.data_ptr(), beams.data_ptr(), words.data_ptr(), ws.data_ptr(), need)
     return top, beams, words
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(*shape: int) -> int:
+    return lib().lq_beam_select_workspace(*shape)

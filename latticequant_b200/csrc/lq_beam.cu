@@ -9,23 +9,27 @@
 // (it decodes greedily, llm/e2e_eval.py:212).
 //
 // Each logit is read once.  Within a beam the order of the totals is the
-// order of the logits, so a slice of a row can give up all but its n best
+// order of the logits, so a part of a row can give up all but its n best
 // before the row's log-sum-exp is known:
-//   beam_slice_kernel  a CTA holds 8192 logits in registers: their maximum
-//       and sum of exponentials, and their n best as sorted keys.  The n
-//       best are found from a bound: among the largest per-thread maxima of
-//       each warp the n-th largest is at most the n-th largest logit, few
-//       logits reach it, and those are ranked by counting.
-//   beam_merge_kernel  a CTA per sequence joins the slices' statistics and
+//   beam_part_kernel  a CTA streams its part of a row through registers, 64
+//       bytes a thread at a time with the next 64 in flight.  Every thread
+//       keeps a maximum and a sum of exponentials of its own.  The n best
+//       are kept by a bound: among the largest per-thread maxima of each warp
+//       of the first tile the n-th largest is at most the n-th best of the
+//       row, few logits reach it, and those are collected in shared memory
+//       and ranked by counting.  A collection that grows past half its room
+//       is cut to its n best, the last of which is the new bound.
+//   beam_merge_kernel  a CTA per sequence joins the parts' statistics and
 //       picks the n best totals the same way.
-// A row with so many equal logits that more than kMaxPicked reach the bound
-// is ranked by n rounds of a block-wide maximum instead.
+// A part with so many equal logits that the collection overflows is ranked by
+// n rounds of a block-wide maximum instead, over the logits in memory.
 #include "lq_attn_common.cuh"
 
 namespace lq {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kPerThread = 32, kSlice = kThreads * kPerThread;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kVecs = 4;  // 16-byte loads of a thread and tile
 constexpr int kMaxPicked = 1024, kMaxN = 128, kMaxBeams = 256, kMaxVocab = 1 << 24;
 
 // Order-preserving image of a float: larger x, larger value; 0 for no
@@ -80,12 +84,13 @@ __device__ __forceinline__ void find_bound(uint32_t best, int n, Picker &s) {
     __syncthreads();
 }
 
-__device__ __forceinline__ void pick(Picker &s, uint32_t hi, uint64_t lo) {
+__device__ __forceinline__ int pick(Picker &s, uint32_t hi, uint64_t lo) {
     const int at = atomicAdd(&s.count, 1);
     if (at < kMaxPicked) {
         s.hi[at] = hi;
         s.lo[at] = lo;
     }
+    return at;
 }
 
 // emit(rank, key) for the n largest picked keys (all distinct); false: too many were picked.
@@ -135,85 +140,174 @@ __device__ void rank_by_rounds(Picker &s, int n, Best best_below, Emit emit) {
     }
 }
 
+// Keep the n best of the s.count <= kMaxPicked picked keys, and make the last of them the bound.
+__device__ __forceinline__ void cut_picked(Picker &s, int n) {
+    const int c = s.count;
+    uint64_t mine[kMaxPicked / kThreads];
+    int at[kMaxPicked / kThreads];
+#pragma unroll
+    for (int q = 0; q < kMaxPicked / kThreads; ++q) {
+        const int i = threadIdx.x + q * kThreads;
+        mine[q] = i < c ? s.lo[i] : 0;
+        at[q] = i < c ? 0 : kMaxPicked;
+        if (i < c)
+            for (int j = 0; j < c; ++j) at[q] += s.lo[j] > mine[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kMaxPicked / kThreads; ++q)
+        if (at[q] < n) {
+            s.lo[at[q]] = mine[q];
+            if (at[q] == n - 1) s.bound = (uint32_t)(mine[q] >> 24);
+        }
+    if (threadIdx.x == 0) s.count = min(c, n);
+    __syncthreads();
+}
+
 struct BeamArgs {
     const void *logits;
     int64_t stride_b, stride_k;
     const float *scores;  // [batch][beams]
-    int beams, vocab, n, slices;
-    float2 *stat;      // [batch * beams][slices]: maximum, sum of exp(x - maximum)
-    uint64_t *keys;    // [batch * beams][slices][n]: ordered(x) << 24 | (2^24 - 1 - word), 0: none
+    int beams, vocab, n, parts, tiles;  // tiles: of a part
+    FastDiv by_beams, by_keys;          // keys: parts * n
+    float2 *stat;      // [batch * beams][parts]: maximum, sum of exp(x - maximum)
+    uint64_t *keys;    // [batch * beams][parts][n]: ordered(x) << 24 | (2^24 - 1 - word), 0: none
     float *top_score;  // [batch][n]
     int64_t *top_beam, *top_word;
 };
 
 constexpr uint64_t kWordMask = (1u << 24) - 1;
 
+__device__ __forceinline__ uint64_t key_of(uint32_t value, int word) {
+    return (uint64_t)value << 24 | (kWordMask - (uint32_t)word);
+}
+
+// Element e of a 16-byte load; a NaN counts as -inf (the maximum with -inf).
 template <int DT>
-__global__ void __launch_bounds__(kThreads) beam_slice_kernel(const __grid_constant__ BeamArgs a) {
+__device__ __forceinline__ float element(const uint32_t (&r)[4], int e) {
+    float f;
+    if constexpr (DT == LQ_F32) f = __uint_as_float(r[e]);
+    else if constexpr (DT == LQ_F16) f = __half2float(__ushort_as_half((uint16_t)(r[e / 2] >> (16 * (e & 1)))));
+    else f = __uint_as_float(e & 1 ? r[e / 2] & 0xffff0000u : r[e / 2] << 16);
+    return fmaxf(f, -INFINITY);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_constant__ BeamArgs a) {
     using T = typename Elem<DT>::T;
-    constexpr int V = 16 / sizeof(T);  // elements of a 16-byte load
+    constexpr int V = 16 / sizeof(T);  // elements of a load
+    constexpr int kTile = kThreads * kVecs * V;
     __shared__ Picker s;
-    __shared__ float red[2 * kWarps];
-    const int row = blockIdx.y, slice = blockIdx.x;
-    const int b = row / a.beams, k = row - b * a.beams;
+    __shared__ float2 red[kWarps];
+    allow_next();
+    const int row = blockIdx.y, part = blockIdx.x;
+    const int b = (int)a.by_beams.div((uint32_t)row), k = row - b * a.beams;
     const T *x0 = static_cast<const T *>(a.logits) + b * a.stride_b + k * a.stride_k;
     // loads start on the 16-byte boundary at or before the row
     const int mis = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
-    const uint4 *base = reinterpret_cast<const uint4 *>(x0 - mis);
-    float x[kPerThread];
-    auto word_of = [&](int j) {  // of x[j]
-        return slice * kSlice + ((j / V) * kThreads + (int)threadIdx.x) * V + j % V - mis;
+    const uint4 *base = reinterpret_cast<const uint4 *>(x0 - mis) + threadIdx.x;
+    const int first = part * a.tiles, last = min(first + a.tiles, (a.vocab + mis + kTile - 1) / kTile);
+    auto word_of = [&](int tile, int i) {  // of element 0 of load i
+        return tile * kTile + (i * kThreads + (int)threadIdx.x) * V - mis;
     };
+    uint32_t none;  // a pair (or one) of -inf
+    if constexpr (DT == LQ_F32) none = 0xff800000u;
+    else if constexpr (DT == LQ_F16) none = 0xfc00fc00u;
+    else none = 0xff80ff80u;
+    auto fetch = [&](int tile, uint4 (&r)[kVecs]) {
 #pragma unroll
-    for (int j = 0; j < kPerThread; j += V) {
-        const int w = word_of(j);
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (w < a.vocab && w + V > 0) u = __ldg(base + (slice * kSlice / V + (j / V) * kThreads + threadIdx.x));
-        const uint32_t r[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            float f;
-            if constexpr (DT == LQ_F32) f = __uint_as_float(r[e]);
-            else if constexpr (DT == LQ_F16) f = __half2float(__ushort_as_half((uint16_t)(r[e / 2] >> (16 * (e & 1)))));
-            else f = __uint_as_float(e & 1 ? r[e / 2] & 0xffff0000u : r[e / 2] << 16);
-            x[j + e] = w + e >= 0 && w + e < a.vocab && f == f ? f : -INFINITY;
+        for (int i = 0; i < kVecs; ++i) {
+            const int w = word_of(tile, i);
+            r[i] = make_uint4(none, none, none, none);
+            if (w < a.vocab && w + V > 0) r[i] = __ldcs(base + (int64_t)tile * (kThreads * kVecs) + i * kThreads);
         }
-    }
-    float mx = x[0];
+    };
+    // words before the row's first and past its last become -inf
+    auto trim = [&](int tile, uint4 (&r)[kVecs]) {
 #pragma unroll
-    for (int j = 1; j < kPerThread; ++j) mx = fmaxf(mx, x[j]);
+        for (int i = 0; i < kVecs; ++i) {
+            const int w = word_of(tile, i);
+            uint32_t u[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (w + e < 0 || w + e >= a.vocab) {
+                    if constexpr (DT == LQ_F32) u[e] = none;
+                    else u[e / 2] = e & 1 ? (u[e / 2] & 0xffffu) | (none & 0xffff0000u)
+                                          : (u[e / 2] & 0xffff0000u) | (none & 0xffffu);
+                }
+            r[i] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    };
 
-    const uint32_t best = ordered(mx);
-    find_bound(best, a.n, s);
-    const uint32_t bound = max(s.bound, 1u);
-    if (best >= bound) {
+    float m = -INFINITY, sum = 0.f;
+    uint4 nx[kVecs];
+    if (threadIdx.x == 0) s.count = 0;
+    if (first < last) fetch(first, nx);
+    bool overflow = false, grown = false;  // the same for the whole block
+    for (int tile = first; tile < last; ++tile) {
+        uint4 cur[kVecs];
 #pragma unroll
-        for (int j = 0; j < kPerThread; ++j)
-            if (ordered(x[j]) >= bound)
-                pick(s, 0u, (uint64_t)ordered(x[j]) << 24 | (kWordMask - (uint32_t)word_of(j)));
+        for (int i = 0; i < kVecs; ++i) cur[i] = nx[i];
+        if (tile + 1 < last) fetch(tile + 1, nx);
+        if (tile * kTile < mis || (tile + 1) * kTile - mis > a.vocab) trim(tile, cur);
+
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const uint32_t u[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+#pragma unroll
+            for (int e = 0; e < V; ++e) mx = fmaxf(mx, element<DT>(u, e));
+        }
+        const uint32_t best = ordered(mx);
+        if (tile == first) find_bound(best, a.n, s);
+        if (grown && !overflow) {
+            overflow = s.count > kMaxPicked;
+            if (!overflow) cut_picked(s, a.n);
+        }
+        int at = 0;
+        const uint32_t bound = max(s.bound, 1u);
+        if (best >= bound && !overflow) {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const uint32_t u[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const uint32_t o = ordered(element<DT>(u, e));
+                    if (o >= bound) at = pick(s, 0u, key_of(o, word_of(tile, i) + e));
+                }
+            }
+        }
+        // the thread's own maximum and sum; finite, so that -inf - m is -inf
+        const float m1 = fmaxf(fmaxf(m, mx), -3.402823466e38f);
+        sum *= exp2f((m - m1) * kLog2e);
+        m = m1;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const uint32_t u[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float y;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((element<DT>(u, e) - m) * kLog2e));
+                sum += y;
+            }
+        }
+        if (tile + 1 < last) grown = __syncthreads_or(at >= kMaxPicked / 2);
     }
 
-    // the slice's maximum and sum of exponentials
-    float top = mx;
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, red[w]);
-    float sum = 0.f;
-    if (top > -INFINITY) {
-#pragma unroll
-        for (int j = 0; j < kPerThread; ++j) sum += exp2f((x[j] - top) * kLog2e);
+    for (int o = 16; o >= 1; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+        const float top = fmaxf(fmaxf(m, m2), -3.402823466e38f);
+        sum = sum * exp2f((m - top) * kLog2e) + s2 * exp2f((m2 - top) * kLog2e);
+        m = top;
     }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((threadIdx.x & 31) == 0) red[kWarps + (threadIdx.x >> 5)] = sum;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(m, sum);
     __syncthreads();
-    const int64_t at = (int64_t)row * a.slices + slice;
+    const int64_t at = (int64_t)row * a.parts + part;
     if (threadIdx.x == 0) {
-        float all = 0.f;
-        for (int w = 0; w < kWarps; ++w) all += red[kWarps + w];
+        float top = red[0].x, all = 0.f;
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, red[w].x);
+        for (int w = 0; w < kWarps; ++w) all += red[w].y * exp2f((red[w].x - top) * kLog2e);
         a.stat[at] = make_float2(top, all);
     }
 
@@ -223,15 +317,23 @@ __global__ void __launch_bounds__(kThreads) beam_slice_kernel(const __grid_const
         rank_by_rounds(
             s, a.n,
             [&](const Key &under) {
-                Key best{0u, 0ull};
+                Key top{0u, 0ull};
+                for (int tile = first; tile < last; ++tile) {
+                    uint4 r[kVecs];
+                    fetch(tile, r);
+                    trim(tile, r);
+                    for (int i = 0; i < kVecs; ++i) {
+                        const uint32_t u[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
 #pragma unroll
-                for (int j = 0; j < kPerThread; ++j) {
-                    const uint32_t o = ordered(x[j]);
-                    const uint64_t lo = o ? (uint64_t)o << 24 | (kWordMask - (uint32_t)word_of(j)) : 0ull;
-                    if (lo < under.lo && lo > best.lo) best.lo = lo;
+                        for (int e = 0; e < V; ++e) {
+                            const uint32_t o = ordered(element<DT>(u, e));
+                            const uint64_t lo = o ? key_of(o, word_of(tile, i) + e) : 0ull;
+                            if (lo < under.lo && lo > top.lo) top.lo = lo;
+                        }
+                    }
                 }
-                best.hi = best.lo ? 1u : 0u;
-                return best;
+                top.hi = top.lo ? 1u : 0u;
+                return top;
             },
             emit);
 }
@@ -240,14 +342,15 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const __grid_const
     __shared__ Picker s;
     __shared__ float lse[kMaxBeams], score[kMaxBeams];
     const int b = blockIdx.x, lane = threadIdx.x & 31;
+    after_previous();
     for (int k = threadIdx.x >> 5; k < a.beams; k += kWarps) {
-        const float2 *st = a.stat + ((int64_t)b * a.beams + k) * a.slices;
+        const float2 *st = a.stat + ((int64_t)b * a.beams + k) * a.parts;
         float m = -INFINITY;
-        for (int i = lane; i < a.slices; i += 32) m = fmaxf(m, st[i].x);
+        for (int i = lane; i < a.parts; i += 32) m = fmaxf(m, st[i].x);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         float sum = 0.f;
-        for (int i = lane; i < a.slices; i += 32)
+        for (int i = lane; i < a.parts; i += 32)
             if (st[i].x > -INFINITY) sum += st[i].y * exp2f((st[i].x - m) * kLog2e);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -257,21 +360,21 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const __grid_const
         }
     }
     __syncthreads();
-    const int per_beam = a.slices * a.n, total = a.beams * per_beam;
+    const int total = a.beams * a.parts * a.n;
     const uint64_t *keys = a.keys + (int64_t)b * total;
-    auto key_of = [&](int i) {
+    auto key_at = [&](int i) {
         const uint64_t lo = keys[i];
-        const int k = i / per_beam;
+        const int k = (int)a.by_keys.div((uint32_t)i);
         const float v = __fadd_rn(__fsub_rn(from_ordered((uint32_t)(lo >> 24)), lse[k]), score[k]);
         return lo ? Key{ordered(v), (uint64_t)(255 - k) << 56 | lo} : Key{0u, 0ull};
     };
     uint32_t best = 0;
-    for (int i = threadIdx.x; i < total; i += kThreads) best = max(best, key_of(i).hi);
+    for (int i = threadIdx.x; i < total; i += kThreads) best = max(best, key_at(i).hi);
     find_bound(best, a.n, s);
     const uint32_t bound = max(s.bound, 1u);
     if (best >= bound)
         for (int i = threadIdx.x; i < total; i += kThreads) {
-            const Key k = key_of(i);
+            const Key k = key_at(i);
             if (k.hi >= bound) pick(s, k.hi, k.lo);
         }
     auto emit = [&](int i, const Key &k) {
@@ -286,7 +389,7 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const __grid_const
             [&](const Key &under) {
                 Key top{0u, 0ull};
                 for (int i = threadIdx.x; i < total; i += kThreads) {
-                    const Key k = key_of(i);
+                    const Key k = key_at(i);
                     if (under > k && k > top) top = k;
                 }
                 return top;
@@ -294,24 +397,34 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const __grid_const
             emit);
 }
 
-int slices_of(int64_t vocab) { return (int)ceil_div(vocab + 7, kSlice); }  // a misaligned row starts up to 7 words in
+// Parts of a row: one resident CTA for each of about four a SM, a tile at least
+// (batches past that stream whole rows).
+struct Plan {
+    int parts, tiles;
+};
 
-bool beam_ok(int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
-    return batch >= 0 && beams >= 1 && beams <= kMaxBeams && vocab >= 1 && vocab <= kMaxVocab && n >= 1 && n <= kMaxN &&
-           batch * beams <= 65535 && beams * slices_of(vocab) * n <= 0x7fffffff;
+Plan plan(int64_t rows, int64_t vocab, int dtype) {
+    const int64_t tile = (int64_t)kThreads * kVecs * (dtype == LQ_F32 ? 4 : 8);
+    const int64_t all = ceil_div(vocab + 7, tile);  // a misaligned row starts up to 7 words in
+    int64_t parts = 148 * 4 / (rows < 1 ? 1 : rows);
+    parts = parts < 1 ? 1 : parts > all ? all : parts;
+    const int64_t tiles = ceil_div(all, parts);
+    return Plan{(int)ceil_div(all, tiles), (int)tiles};
 }
 
-size_t stat_bytes(int64_t rows, int slices) { return (size_t)rows * slices * sizeof(float2); }
+bool beam_ok(int64_t batch, int64_t beams, int64_t vocab, int64_t n, int dtype) {
+    return batch >= 0 && beams >= 1 && beams <= kMaxBeams && vocab >= 1 && vocab <= kMaxVocab && n >= 1 && n <= kMaxN &&
+           batch <= 65535 && batch * beams <= 65535 && (dtype == LQ_F32 || dtype == LQ_F16 || dtype == LQ_BF16);
+}
 
 }  // namespace
 }  // namespace lq
 
 using namespace lq;
 
-extern "C" size_t lq_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
-    if (!beam_ok(batch, beams, vocab, n)) return 0;
-    const int64_t rows = batch * beams;
-    return stat_bytes(rows, slices_of(vocab)) + (size_t)rows * slices_of(vocab) * n * 8;
+extern "C" size_t lq_beam_select_workspace(int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
+    if (!beam_ok(batch, beams, vocab, n, dtype)) return 0;
+    return (size_t)batch * beams * plan(batch * beams, vocab, dtype).parts * (sizeof(float2) + 8 * n);
 }
 
 extern "C" int lq_beam_select(const void *logits, int dtype, int64_t batch, int64_t beams, int64_t vocab,
@@ -319,10 +432,11 @@ extern "C" int lq_beam_select(const void *logits, int dtype, int64_t batch, int6
                               int64_t *top_beam, int64_t *top_word, void *workspace, size_t workspace_bytes,
                               void *stream) {
     LQ_NVTX_RANGE();
-    if (!beam_ok(batch, beams, vocab, n)) return LQ_ERR_INVALID;
+    if (!beam_ok(batch, beams, vocab, n, dtype)) return LQ_ERR_INVALID;
     if (batch == 0) return LQ_OK;
     if (!logits || !scores || !top_score || !top_beam || !top_word || !workspace) return LQ_ERR_INVALID;
-    if (workspace_bytes < lq_beam_select_workspace(batch, beams, vocab, n)) return LQ_ERR_CAPACITY;
+    if (workspace_bytes < lq_beam_select_workspace(dtype, batch, beams, vocab, n)) return LQ_ERR_CAPACITY;
+    const Plan p = plan(batch * beams, vocab, dtype);
     BeamArgs a{};
     a.logits = logits;
     a.stride_b = stride_b;
@@ -331,19 +445,20 @@ extern "C" int lq_beam_select(const void *logits, int dtype, int64_t batch, int6
     a.beams = (int)beams;
     a.vocab = (int)vocab;
     a.n = (int)n;
-    a.slices = slices_of(vocab);
+    a.parts = p.parts;
+    a.tiles = p.tiles;
+    a.by_beams = FastDiv((uint32_t)beams);
+    a.by_keys = FastDiv((uint32_t)(p.parts * n));
     a.stat = static_cast<float2 *>(workspace);
-    a.keys = reinterpret_cast<uint64_t *>(static_cast<char *>(workspace) + stat_bytes(batch * beams, a.slices));
+    a.keys = reinterpret_cast<uint64_t *>(a.stat + batch * beams * p.parts);
     a.top_score = top_score;
     a.top_beam = top_beam;
     a.top_word = top_word;
     cudaStream_t st = as_stream(stream);
-    const dim3 grid((unsigned)a.slices, (unsigned)(batch * beams));
-    if (dtype == LQ_F32) beam_slice_kernel<LQ_F32><<<grid, kThreads, 0, st>>>(a);
-    else if (dtype == LQ_F16) beam_slice_kernel<LQ_F16><<<grid, kThreads, 0, st>>>(a);
-    else if (dtype == LQ_BF16) beam_slice_kernel<LQ_BF16><<<grid, kThreads, 0, st>>>(a);
-    else return LQ_ERR_INVALID;
+    const dim3 grid((unsigned)p.parts, (unsigned)(batch * beams));
+    if (dtype == LQ_F32) beam_part_kernel<LQ_F32><<<grid, kThreads, 0, st>>>(a);
+    else if (dtype == LQ_F16) beam_part_kernel<LQ_F16><<<grid, kThreads, 0, st>>>(a);
+    else beam_part_kernel<LQ_BF16><<<grid, kThreads, 0, st>>>(a);
     if (check_launch() != LQ_OK) return LQ_ERR_CUDA;
-    beam_merge_kernel<<<(unsigned)batch, kThreads, 0, st>>>(a);
-    return check_launch();
+    return launch_overlapped(beam_merge_kernel, dim3((unsigned)batch), kThreads, 0, st, a);
 }

@@ -23,6 +23,29 @@ inline int check_launch() {
     return e == cudaSuccess ? LQ_OK : LQ_ERR_CUDA;
 }
 
+// Launch a kernel that may begin while the stream's previous kernel drains
+// (programmatic stream serialisation): it must call after_previous() before it
+// touches what that kernel writes.
+template <class... Params, class... Args>
+inline int launch_overlapped(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
+                             Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at = {};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, Params(args)...) == cudaSuccess ? check_launch() : LQ_ERR_CUDA;
+}
+// Waits until the previous kernel of the stream has finished and its writes are visible.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next kernel's CTAs be scheduled once every CTA of this one got here or ended.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 inline cudaStream_t as_stream(void *s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // One NVTX range per C entry point that enqueues work, named after the

@@ -20,13 +20,14 @@ into ``err``, a (1,) int32 device tensor, for ``_lib.raise_flags``.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr, stream_handle
+from ._lib import call, lib
 
 _I32, _F32 = torch.int32, torch.float32
 
@@ -43,26 +44,38 @@ def empty_pool(n_layers: int, n_pages: int, n_heads: int, head_dim: int, page_to
 
 
 def _pool(codes: torch.Tensor, scales: torch.Tensor, dims: int):
-    """The pool's shape after its layer dimension, checked."""
-    _lib.require_cuda(codes)
-    shape = codes.shape
-    if len(shape) != dims or codes.dtype != _I32 or scales.dtype != _F32 or scales.shape != shape[:-1] or \
-            shape[-4] != 2 or not (codes.is_contiguous() and scales.is_contiguous()) or scales.device != codes.device:
+    """(device index, n_pages, heads, page_tokens, head_dim) of a pool or one of its layers, checked."""
+    if not codes.is_cuda:
+        _lib.require_cuda(codes)
+    shape, index = codes.shape, codes.get_device()
+    if len(shape) != dims or shape[-4] != 2 or codes.dtype is not _I32 or not codes.is_contiguous() or \
+            _wrong(scales, _F32, shape[:-1], index):
         raise ValueError("a page pool is contiguous int32 codes " + ("(layers, " if dims == 6 else "(") +
                          "n_pages, 2, heads, page_tokens, head_dim / 8) with fp32 scales of the same leading shape")
     if shape[-1] not in (8, 16) or shape[-2] not in (16, 32, 64, 128, 256):
         raise ValueError("a page pool takes head_dim 64 or 128 and pages of 16, 32, 64, 128 or 256 tokens")
-    return shape[-5], shape[-3], shape[-2], shape[-1] * 8
+    return index, shape[-5], shape[-3], shape[-2], shape[-1] * 8
 
 
-def _index(t: torch.Tensor, dtype, shape, name: str, device):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+def _wrong(t: torch.Tensor, dtype, shape, index: int) -> bool:
+    return t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous()
+
+
+def _need(t: torch.Tensor, dtype, shape, name: str, index: int) -> int:
+    """The address of t, which must be contiguous, of this dtype, shape and device."""
+    if _wrong(t, dtype, shape, index):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{index}")
+    return t.data_ptr()
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with a contiguous last dimension, 16-byte aligned, its other strides multiples of 8 elements."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+    *outer, last = t.stride()
+    if last == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in outer):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -75,22 +88,20 @@ def append(codes: torch.Tensor, scales: torch.Tensor, k: torch.Tensor, v: torch.
     int64 (n,): page * page_tokens + row, distinct, negative: not stored.  With
     ``dequantised`` returns the stored values (k, v) in the inputs' dtype, as
     CompressedKVCache.update() does, else None."""
-    n_pages, H, P, D = _pool(codes, scales, 5)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (H, D) or k.dtype != v.dtype or \
-            k.device != codes.device or v.device != codes.device:
+    index, n_pages, H, P, D = _pool(codes, scales, 5)
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != H or shape[2] != D or v.shape != shape or k.dtype is not v.dtype or \
+            k.get_device() != index or v.get_device() != index:
         raise ValueError(f"k and v must be (n, {H}, {D}) tensors of one dtype on the pool's device")
-    n = k.shape[0]
-    _index(slots, torch.int64, (n,), "slots", codes.device)
-    dt = _lib.dtype_code(k.dtype)
+    n = shape[0]
+    slots_p, dt = _need(slots, torch.int64, (n,), "slots", index), _lib.dtype_code(k.dtype)
     k, v = _rows(k), _rows(v)
     ko = vo = None
     if dequantised:
-        ko, vo = torch.empty((n, H, D), dtype=k.dtype, device=k.device), torch.empty((n, H, D), dtype=k.dtype,
-                                                                                   device=k.device)
-    with torch.cuda.device(codes.device):
-        check(lib().lq_paged_append(ptr(k), ptr(v), dt, n, H, D, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                                    ptr(slots), n_pages, P, ptr(codes), ptr(scales), ptr(ko), ptr(vo), ptr(err),
-                                    stream_handle(codes.device)), "lq_paged_append")
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        vo = torch.empty_like(ko)
+    call("lq_paged_append", index, k.data_ptr(), v.data_ptr(), dt, n, H, D, *k.stride()[:2], *v.stride()[:2], slots_p,
+         n_pages, P, codes.data_ptr(), scales.data_ptr(), _ptr(ko), _ptr(vo), _ptr(err))
     return (ko, vo) if dequantised else None
 
 
@@ -109,38 +120,41 @@ def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, t
     the table's width), which sets the split.  Returns o (B, Hq, T, D) in q's
     dtype (and the fp32 (B, Hq, T) log-sum-exp if return_lse); a position that
     sees nothing gives 0 and -inf."""
-    n_pages, H, P, D = _pool(codes, scales, 5)
-    dev = codes.device
-    if q.dim() != 4 or q.shape[3] != D or q.shape[1] % H or q.shape[1] == 0 or q.shape[2] == 0 or q.device != dev:
-        raise ValueError(f"q must be (B, Hq, T, {D}) with Hq a multiple of {H}, on the pool's device")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"tree_attention takes float16 or bfloat16 queries, not {q.dtype}")
-    B, Hq, T, _ = q.shape
-    if table.dim() != 2 or table.shape[0] != B:
-        raise ValueError(f"table must hold {B} rows")
-    _index(table, _I32, table.shape, "table", dev)
-    _index(lens, _I32, (B,), "lens", dev)
-    mask_stride = 0
+    index, n_pages, H, P, D = _pool(codes, scales, 5)
+    if q.dim() != 4 or q.get_device() != index:
+        raise ValueError(f"q must be (B, Hq, T, {D}) on the pool's device")
+    B, Hq, T, d = q.shape
+    if d != D or Hq % H or Hq == 0 or T == 0:
+        raise ValueError(f"q must be (B, Hq, T, {D}) with Hq a multiple of {H} and T at least 1")
+    dtype = q.dtype
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise ValueError(f"tree_attention takes float16 or bfloat16 queries, not {dtype}")
+    width = table.shape[1] if table.dim() == 2 else -1
+    table_p, lens_p = _need(table, _I32, (B, width), "table", index), _need(lens, _I32, (B,), "lens", index)
+    mask_p, mask_stride = None, 0
     if mask is not None:
-        _index(mask, torch.bool, (B, T, T) if mask.dim() == 3 else (T, T), "mask", dev)
-        mask_stride = T * T if mask.dim() == 3 else 0
+        per_row = mask.dim() == 3
+        mask_p = _need(mask, torch.bool, (B, T, T) if per_row else (T, T), "mask", index)
+        mask_stride = T * T if per_row else 0
     q = _rows(q)
     if out is None:
-        out = torch.empty((B, Hq, T, D), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _index(out, q.dtype, (B, Hq, T, D), "out", dev)
-    lse = torch.empty((B, Hq, T), dtype=_F32, device=dev) if return_lse else None
-    width = table.shape[1]
+        _need(out, dtype, (B, Hq, T, D), "out", index)
+    lse = lens.new_empty((B, Hq, T), dtype=_F32) if return_lse else None
     bound = width * P if max_len is None else min(int(max_len), width * P)
-    with torch.cuda.device(dev):
-        need = lib().lq_paged_attention_workspace(B, H, Hq // H, T, D, bound)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        check(lib().lq_paged_attention(ptr(q), _lib.dtype_code(q.dtype), q.stride(0), q.stride(1), q.stride(2),
-                                       ptr(codes), ptr(scales), n_pages, P, ptr(table), width, width, ptr(lens), bound,
-                                       ptr(mask), mask_stride, B, H, Hq // H, T, D,
-                                       1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), ptr(out), ptr(lse),
-                                       ptr(ws), need, ptr(err), stream_handle(dev)), "lq_paged_attention")
+    need = _attention_workspace(B, H, Hq // H, T, D, bound)
+    ws = codes.new_empty(need // 4) if need else None
+    call("lq_paged_attention", index, q.data_ptr(), _lib.dtype_code(dtype), *q.stride()[:3], codes.data_ptr(),
+         scales.data_ptr(), n_pages, P, table_p, width, width, lens_p, bound, mask_p, mask_stride, B, H, Hq // H, T, D,
+         1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), out.data_ptr(), _ptr(lse), _ptr(ws), need,
+         _ptr(err))
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(*shape: int) -> int:
+    return lib().lq_paged_attention_workspace(*shape)
 
 
 def fork_pages(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor,
@@ -154,24 +168,21 @@ def fork_pages(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, l
     that no child names are freed.  parents = arange reserves, parents with -1
     entries free rows, repeated parents fork: beam search's reordering is
     parents = the selected beams."""
-    n_pages, H, P, D = _pool(codes, scales, 6)
-    dev = codes.device
+    index, n_pages, H, P, D = _pool(codes, scales, 6)
     if table.dim() != 2 or parents.dim() != 1:
         raise ValueError("table is (rows, width) and parents (children,)")
     (rows, width), n = table.shape, parents.shape[0]
-    _index(table, _I32, (rows, width), "table", dev)
-    _index(lens, _I32, (rows,), "lens", dev)
-    _index(refs, _I32, (n_pages,), "refs", dev)
-    _index(parents, torch.int64, (n,), "parents", dev)
-    new = (torch.empty((n, width), dtype=_I32, device=dev), torch.empty(n, dtype=_I32, device=dev),
-           torch.empty(n_pages, dtype=_I32, device=dev))
-    with torch.cuda.device(dev):
-        need = lib().lq_pages_fork_workspace(rows, n, n_pages)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        check(lib().lq_pages_fork(ptr(table), rows, width, ptr(lens), ptr(refs), ptr(parents), n, int(reserve),
-                                  *(ptr(t) for t in new), ptr(codes), ptr(scales), codes.shape[0], n_pages, H, P, D,
-                                  ptr(ws), need, ptr(err), stream_handle(dev)), "lq_pages_fork")
-    return new
+    table_p, lens_p = _need(table, _I32, (rows, width), "table", index), _need(lens, _I32, (rows,), "lens", index)
+    refs_p, parents_p = _need(refs, _I32, (n_pages,), "refs", index), _need(parents, torch.int64, (n,), "parents", index)
+    new_table = table.new_empty((n, width))
+    new_lens = lens.new_empty(n)
+    new_refs = torch.empty_like(refs)
+    need = 4 * (rows + n + n_pages)  # lq_pages_fork_workspace
+    ws = refs.new_empty(need // 4)
+    call("lq_pages_fork", index, table_p, rows, width, lens_p, refs_p, parents_p, n, int(reserve), new_table.data_ptr(),
+         new_lens.data_ptr(), new_refs.data_ptr(), codes.data_ptr(), scales.data_ptr(), codes.shape[0], n_pages, H, P, D,
+         ws.data_ptr(), need, _ptr(err))
+    return new_table, new_lens, new_refs
 
 
 def compact_pages(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, refs: torch.Tensor,
@@ -179,18 +190,14 @@ def compact_pages(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor
     """Move the live pages to the front of the pool (lq_pages_compact): (table,
     refs, n_live), n_live a (1,) int32 device tensor.  ``table`` holds every
     entry that names a page (any shape)."""
-    n_pages, H, P, D = _pool(codes, scales, 6)
-    dev = codes.device
-    _index(table, _I32, table.shape, "table", dev)
-    _index(refs, _I32, (n_pages,), "refs", dev)
-    new_table, new_refs = torch.empty_like(table), torch.empty_like(refs)
-    n_live = torch.empty(1, dtype=_I32, device=dev)
-    with torch.cuda.device(dev):
-        need = lib().lq_pages_compact_workspace(n_pages)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        check(lib().lq_pages_compact(ptr(table), table.numel(), ptr(refs), ptr(new_table), ptr(new_refs), ptr(n_live),
-                                     ptr(codes), ptr(scales), codes.shape[0], n_pages, H, P, D, ptr(ws), need, ptr(err),
-                                     stream_handle(dev)), "lq_pages_compact")
+    index, n_pages, H, P, D = _pool(codes, scales, 6)
+    table_p, refs_p = _need(table, _I32, table.shape, "table", index), _need(refs, _I32, (n_pages,), "refs", index)
+    new_table, new_refs, n_live = torch.empty_like(table), torch.empty_like(refs), refs.new_empty(1)
+    need = 12 * n_pages + 4  # lq_pages_compact_workspace
+    ws = refs.new_empty(need // 4)
+    call("lq_pages_compact", index, table_p, table.numel(), refs_p, new_table.data_ptr(), new_refs.data_ptr(),
+         n_live.data_ptr(), codes.data_ptr(), scales.data_ptr(), codes.shape[0], n_pages, H, P, D, ws.data_ptr(), need,
+         _ptr(err))
     return new_table, new_refs, n_live
 
 
@@ -199,17 +206,13 @@ def copy_pages(codes: torch.Tensor, scales: torch.Tensor, src: torch.Tensor, dst
     """Copy pages src[i] to dst[i] in all layers (lq_pages_copy); no page is both
     a source and a destination, and no destination is named twice.  ``count``, a
     (1,) int32 device tensor, limits the pairs."""
-    n_pages, H, P, D = _pool(codes, scales, 6)
-    dev = codes.device
+    index, n_pages, H, P, D = _pool(codes, scales, 6)
     n = src.numel()
-    _index(src, _I32, (n,), "src", dev)
-    _index(dst, _I32, (n,), "dst", dev)
+    src_p, dst_p = _need(src, _I32, (n,), "src", index), _need(dst, _I32, (n,), "dst", index)
     if count is None:
-        count = torch.full((1,), n, dtype=_I32, device=dev)
-    _index(count, _I32, (1,), "count", dev)
-    with torch.cuda.device(dev):
-        check(lib().lq_pages_copy(ptr(src), ptr(dst), ptr(count), n, ptr(codes), ptr(scales), codes.shape[0], n_pages, H,
-                                  P, D, ptr(err), stream_handle(dev)), "lq_pages_copy")
+        count = torch.full((1,), n, dtype=_I32, device=src.device)
+    call("lq_pages_copy", index, src_p, dst_p, _need(count, _I32, (1,), "count", index), n, codes.data_ptr(),
+         scales.data_ptr(), codes.shape[0], n_pages, H, P, D, _ptr(err))
 
 
 def accept_tokens(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, n_draft: int,
@@ -219,17 +222,13 @@ def accept_tokens(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor
     accepted int32 (rows, most): draft indices, strictly ascending (a path of
     the tree from its root), padded with -1.  Their rows move to the front of
     the drafts' slots in all layers.  Returns the new lens."""
-    n_pages, H, P, D = _pool(codes, scales, 6)
-    dev = codes.device
+    index, n_pages, H, P, D = _pool(codes, scales, 6)
     if table.dim() != 2 or accepted.dim() != 2:
         raise ValueError("table is (rows, width) and accepted (rows, most)")
     (rows, width), most = table.shape, accepted.shape[1]
-    _index(table, _I32, (rows, width), "table", dev)
-    _index(lens, _I32, (rows,), "lens", dev)
-    _index(accepted, _I32, (rows, most), "accepted", dev)
+    table_p, lens_p = _need(table, _I32, (rows, width), "table", index), _need(lens, _I32, (rows,), "lens", index)
+    accepted_p = _need(accepted, _I32, (rows, most), "accepted", index)
     new_lens = torch.empty_like(lens)
-    with torch.cuda.device(dev):
-        check(lib().lq_pages_accept(ptr(table), rows, width, ptr(lens), int(n_draft), ptr(accepted), most,
-                                    ptr(new_lens), ptr(codes), ptr(scales), codes.shape[0], n_pages, H, P, D, ptr(err),
-                                    stream_handle(dev)), "lq_pages_accept")
+    call("lq_pages_accept", index, table_p, rows, width, lens_p, int(n_draft), accepted_p, most, new_lens.data_ptr(),
+         codes.data_ptr(), scales.data_ptr(), codes.shape[0], n_pages, H, P, D, _ptr(err))
     return new_lens
