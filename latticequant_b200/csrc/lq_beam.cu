@@ -17,8 +17,8 @@
 //       are kept by a bound: among the largest per-thread maxima of each warp
 //       of the first tile the n-th largest is at most the n-th best of the
 //       row, few logits reach it, and those are collected in shared memory
-//       and ranked by counting.  A collection that grows past half its room
-//       is cut to its n best, the last of which is the new bound.
+//       and ranked by counting.  A collection of more than 2 n is cut to its
+//       n best, the last of which is the new bound.
 //   beam_merge_kernel  a CTA per sequence joins the parts' statistics and
 //       picks the n best totals the same way.
 // A part with so many equal logits that the collection overflows is ranked by
@@ -182,14 +182,37 @@ __device__ __forceinline__ uint64_t key_of(uint32_t value, int word) {
     return (uint64_t)value << 24 | (kWordMask - (uint32_t)word);
 }
 
-// Element e of a 16-byte load; a NaN counts as -inf (the maximum with -inf).
+// Element e of a 16-byte load.
 template <int DT>
 __device__ __forceinline__ float element(const uint32_t (&r)[4], int e) {
-    float f;
-    if constexpr (DT == LQ_F32) f = __uint_as_float(r[e]);
-    else if constexpr (DT == LQ_F16) f = __half2float(__ushort_as_half((uint16_t)(r[e / 2] >> (16 * (e & 1)))));
-    else f = __uint_as_float(e & 1 ? r[e / 2] & 0xffff0000u : r[e / 2] << 16);
-    return fmaxf(f, -INFINITY);
+    if constexpr (DT == LQ_F32) return __uint_as_float(r[e]);
+    else if constexpr (DT == LQ_F16) return __half2float(__ushort_as_half((uint16_t)(r[e / 2] >> (16 * (e & 1)))));
+    else return __uint_as_float(e & 1 ? r[e / 2] & 0xffff0000u : r[e / 2] << 16);
+}
+
+// The largest element of a 16-byte load, NaNs aside (two at a time in 16 bits).
+template <int DT>
+__device__ __forceinline__ float largest(const uint4 &v) {
+    if constexpr (DT == LQ_F32) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    } else {
+        uint32_t r[3];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const uint32_t p = i < 2 ? w[2 * i] : r[0], q = i < 2 ? w[2 * i + 1] : r[1];
+            if constexpr (DT == LQ_F16) asm("max.f16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(p), "r"(q));
+            else asm("max.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(p), "r"(q));
+        }
+        const uint32_t pair[4] = {r[2], 0u, 0u, 0u};
+        return fmaxf(element<DT>(pair, 0), element<DT>(pair, 1));
+    }
+}
+
+__device__ __forceinline__ float exp_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 template <int DT>
@@ -244,6 +267,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
     if (threadIdx.x == 0) s.count = 0;
     if (first < last) fetch(first, nx);
     bool overflow = false, grown = false;  // the same for the whole block
+    const int cut_at = 2 * a.n;
     for (int tile = first; tile < last; ++tile) {
         uint4 cur[kVecs];
 #pragma unroll
@@ -251,12 +275,11 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
         if (tile + 1 < last) fetch(tile + 1, nx);
         if (tile * kTile < mis || (tile + 1) * kTile - mis > a.vocab) trim(tile, cur);
 
-        float mx = -INFINITY;
+        float top[kVecs], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
-            const uint32_t u[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
-#pragma unroll
-            for (int e = 0; e < V; ++e) mx = fmaxf(mx, element<DT>(u, e));
+            top[i] = largest<DT>(cur[i]);
+            mx = fmaxf(mx, top[i]);
         }
         const uint32_t best = ordered(mx);
         if (tile == first) find_bound(best, a.n, s);
@@ -269,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
         if (best >= bound && !overflow) {
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
+                if (ordered(top[i]) < bound) continue;
                 const uint32_t u[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
@@ -277,21 +301,37 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
                 }
             }
         }
-        // the thread's own maximum and sum; finite, so that -inf - m is -inf
+        // the thread's own maximum and sum; the maximum finite, so that -inf - m is -inf
         const float m1 = fmaxf(fmaxf(m, mx), -3.402823466e38f);
         sum *= exp2f((m - m1) * kLog2e);
         m = m1;
+        const unsigned long long minus = f2_pack(-m, -m), scale = f2_pack(kLog2e, kLog2e);
+        unsigned long long acc = 0;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
             const uint32_t u[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float y;
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((element<DT>(u, e) - m) * kLog2e));
-                sum += y;
+            for (int e = 0; e < V; e += 2) {
+                float y0, y1;
+                f2_unpack(f2_mul(f2_add(f2_pack(element<DT>(u, e), element<DT>(u, e + 1)), minus), scale), y0, y1);
+                acc = f2_add(acc, f2_pack(exp_of(y0), exp_of(y1)));
             }
         }
-        if (tile + 1 < last) grown = __syncthreads_or(at >= kMaxPicked / 2);
+        float a0, a1;
+        f2_unpack(acc, a0, a1);
+        a0 += a1;
+        if (a0 != a0) {  // a NaN logit (left out), or +inf (stays NaN)
+            a0 = 0.f;
+#pragma unroll 1
+            for (int i = 0; i < kVecs; ++i) {
+                const uint4 c = i == 0 ? cur[0] : i == 1 ? cur[1] : i == 2 ? cur[2] : cur[3];
+                const uint32_t u[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                for (int e = 0; e < V; ++e) a0 += exp_of((fmaxf(element<DT>(u, e), -INFINITY) - m) * kLog2e);
+            }
+        }
+        sum += a0;
+        if (tile + 1 < last) grown = __syncthreads_or(at >= cut_at);
     }
 
 #pragma unroll

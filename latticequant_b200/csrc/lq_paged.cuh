@@ -20,48 +20,80 @@ namespace lq {
 __host__ __device__ constexpr bool paged_page_ok(int p) { return p >= 16 && p <= 256 && (p & (p - 1)) == 0; }
 __host__ __device__ constexpr bool paged_dim_ok(int d) { return d == 64 || d == 128; }
 
-// A code word ready for extraction: nibble 7 - i of `w` is u_i, `magic` the
-// floating-point constant that carries the coset's half.
-struct CodeWord {
-    uint32_t w, magic;
-};
+// ---- block decode -----------------------------------------------------------
+// A word's eight 4-bit fields become four fp16 pairs by one logic op and one
+// exact fp16 op each: a field lands in the mantissa of 1024, either at bits
+// 1-4 (value 1024 + 2u + coset, then -1040) or at bits 5-8 (1024 + 32u + 16
+// coset, then /16 - 80), so that one right shift serves both pairs of half
+// the word.  Every pair comes out as 2 * (u - 8) + coset, exact.  What bounds
+// the kernels is the integer ALU pipe; left shifts, the coset's constants and
+// the top bit are written as multiplications, which run on the FMA pipe.
+constexpr float kCodeUnit = 0.5f;  // what one unit of the decoded pairs stands for
 
-// `w` regains u7's low bit: with the coset bit shifted out, the parity of
-// u0..u6 is the population of their low bits (bits 4, 8, .. 28).
-template <bool BF16>
-__device__ __forceinline__ CodeWord code_word(uint32_t v) {
-    CodeWord c;
-    const uint32_t t = v << 1;
-    c.w = t | (__popc(t & 0x11111110u) & 1);
-    const uint32_t half = v >> 31;
-    // fp16: 1024 + 16 u + 8 coset (unit 1 in the mantissa); bf16: 128 + 2 u + coset
-    c.magic = BF16 ? half * 0x00010001u + 0x43004300u : half * 0x00080008u + 0x64006400u;
-    return c;
+constexpr uint32_t kField1 = 0x001e001eu, kField5 = 0x01e001e0u;  // fields at bits 1-4 and 5-8 of each half
+
+__device__ __forceinline__ uint32_t pair_at1(uint32_t x, uint32_t magic) {
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((x & kField1) | magic), "r"(0xe410e410u));  // - (1024 + 16)
+    return r;
+}
+__device__ __forceinline__ uint32_t pair_at5(uint32_t x, uint32_t magic) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;"
+        : "=r"(r)
+        : "r"((x & kField5) | magic), "r"(0x2c002c00u), "r"(0xd500d500u));  // * 1/16 - (64 + 16)
+    return r;
 }
 
-// Channels (7 - S, 3 - S) of the block as a packed pair, in units of 1/16
-// (fp16) or 1/2 (bf16): one shift, one three-input logic op and one exact
-// subtraction for two channels.
-template <bool BF16, int S>
-__device__ __forceinline__ uint32_t code_pair(const CodeWord &c) {
-    if constexpr (BF16) {
-        const uint32_t x = S == 0 ? c.w << 1 : c.w >> (4 * S - 1);
-        const uint32_t y = (x & 0x001e001eu) | c.magic;
-        const uint32_t off = 0xc310c310u;  // -(128 + 16)
-        uint32_t r;
-        asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(y), "r"(off));
-        return r;
+// The low bit of u7, shifted out of the word: the parity of u0..u6.
+__device__ __forceinline__ uint32_t odd_sum(uint32_t v) { return (uint32_t)__popc(v & 0x08888888u); }  // bit 0
+
+// The pairs of one block: pair s holds channels 7 - s (low half) and 3 - s.
+__device__ __forceinline__ void decode_block(uint32_t v, uint32_t (&pair)[4]) {
+    const uint32_t a = ((odd_sum(v) * 2u) & 2u) | (v * 4u);  // u7, u6 | u3, u2 at bits 1-8 of the halves
+    const uint32_t b = v >> 6;                               // u5, u4 | u1, u0
+    const uint32_t half = __umulhi(v, 2u);                   // the coset
+    const uint32_t m1 = half * 0x00010001u + 0x64006400u, m5 = half * 0x00100010u + 0x64006400u;
+    pair[0] = pair_at1(a, m1);
+    pair[1] = pair_at5(a, m5);
+    pair[2] = pair_at1(b, m1);
+    pair[3] = pair_at5(b, m5);
+}
+
+// The pairs of one block of two tokens: low[s] holds channel 7 - s of token x
+// (low half) and of token y, high[s] channel 3 - s of both.
+struct TokenPair {
+    uint32_t la, lb, ha, hb, m1, m5;
+};
+__device__ __forceinline__ TokenPair pair_tokens(uint32_t x, uint32_t y) {
+    const uint32_t tx = x * 2u, ty = y * 2u;
+    const uint32_t l = __byte_perm(tx, ty, 0x5410), h = __byte_perm(tx, ty, 0x7632);
+    const uint32_t odd = odd_sum(y) * 0x20000u + odd_sum(x) * 2u;
+    const uint32_t half = __umulhi(y, 2u) * 0x10000u + __umulhi(x, 2u);
+    TokenPair p;
+    p.la = (odd & 0x00020002u) | (l * 2u);
+    p.lb = l >> 7;
+    p.ha = h * 2u;
+    p.hb = h >> 7;
+    p.m1 = half + 0x64006400u;
+    p.m5 = half * 16u + 0x64006400u;
+    return p;
+}
+template <int S>
+__device__ __forceinline__ void decode_pair(const TokenPair &p, uint32_t &low, uint32_t &high) {
+    if constexpr (S == 0) {
+        low = pair_at1(p.la, p.m1);
+        high = pair_at1(p.ha, p.m1);
+    } else if constexpr (S == 1) {
+        low = pair_at5(p.la, p.m5);
+        high = pair_at5(p.ha, p.m5);
+    } else if constexpr (S == 2) {
+        low = pair_at1(p.lb, p.m1);
+        high = pair_at1(p.hb, p.m1);
     } else {
-        const uint32_t x = S == 0 ? c.w << 4 : S == 1 ? c.w : c.w >> (4 * S - 4);
-        const uint32_t y = (x & 0x00f000f0u) | c.magic;
-        const uint32_t off = 0xe480e480u;  // -(1024 + 128)
-        uint32_t r;
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(y), "r"(off));
-        return r;
+        low = pair_at5(p.lb, p.m5);
+        high = pair_at5(p.hb, p.m5);
     }
 }
-
-template <bool BF16>
-constexpr float kCodeUnit = BF16 ? 0.5f : 0.0625f;  // what one unit of code_pair's values stands for
 
 }  // namespace lq

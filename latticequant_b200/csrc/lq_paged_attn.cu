@@ -11,8 +11,10 @@
 // Mathematics.  A query row r = t * G + g; the tile of a warp is 16 tokens by
 // 8 * NT rows.  Scores S = K Q^T put tokens on the rows of the MMA, so a
 // lane's A registers are whole code words of "its" two tokens, decoded in
-// registers: values are exact in q's own type (fp16 or bf16) and the token's
-// scale multiplies the fp32 score.  V's scale goes into the exponent:
+// registers to fp16, which holds every point exactly.  A bf16 query becomes
+// fp16 times a power of two of its row (its largest value then lies in
+// [2^10, 2^11); what falls under fp16's smallest step is 2^-35 of that), and
+// the token's and the row's factors multiply the fp32 score.  V's scale goes into the exponent:
 //   x = s * log2(e) * sm_scale * ks + log2(vs),  w = 2^(x - M),
 //   o += w * point,  l += w / vs
 // so the fp16 weights w stay within 2^14 whatever the scales are.  M is a
@@ -28,17 +30,11 @@ namespace {
 
 constexpr int kWarps = 4;
 
-template <bool BF16>
 __device__ __forceinline__ void mma_16816(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
-    if constexpr (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
@@ -95,36 +91,33 @@ __device__ __forceinline__ void load_tile(const PagedAttnArgs &a, const uint32_t
         load_words<Tile<D>::VW>(vp + (2 * t + (i & 1) + 8 * (i >> 1)) * W + g * Tile<D>::VW, x.v[i]);
 }
 
-// Both 16-bit halves of two registers, regrouped: lo = (a.lo, b.lo), hi = (a.hi, b.hi).
-__device__ __forceinline__ void zip_halves(uint32_t a, uint32_t b, uint32_t &lo, uint32_t &hi) {
-    lo = __byte_perm(a, b, 0x5410);
-    hi = __byte_perm(a, b, 0x7632);
-}
-
+// v[block][half]: tokens 2t, 2t+1 (+ 8 half) of this lane's blocks
 template <int D, int NT, int S>
-__device__ __forceinline__ void pv_step(const CodeWord c[4][D / 64], const uint32_t (*p)[2], float (*o)[NT][4]) {
+__device__ __forceinline__ void pv_step(const TokenPair v[D / 64][2], const uint32_t (*p)[2], float (*o)[NT][4]) {
     if constexpr (D == 128) {
-        uint32_t a[4], b[4];  // [block * 2 + token group] for the pair's two channels
+        uint32_t a[4], b[4];  // [block + 2 half] of the pair's two channels
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-                zip_halves(code_pair<false, S>(c[2 * half][blk]), code_pair<false, S>(c[2 * half + 1][blk]),
-                           a[blk + 2 * half], b[blk + 2 * half]);
+            for (int half = 0; half < 2; ++half) decode_pair<S>(v[blk][half], a[blk + 2 * half], b[blk + 2 * half]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            mma_16816<false>(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
-            mma_16816<false>(o[4 + S][n], b[0], b[1], b[2], b[3], p[n][0], p[n][1]);
+            mma_16816(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
+            mma_16816(o[4 + S][n], b[0], b[1], b[2], b[3], p[n][0], p[n][1]);
         }
     } else {
         uint32_t a[4];  // one block: its two channels are the MMA's two row groups
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-            zip_halves(code_pair<false, S>(c[2 * half][0]), code_pair<false, S>(c[2 * half + 1][0]), a[2 * half],
-                       a[1 + 2 * half]);
+        for (int half = 0; half < 2; ++half) decode_pair<S>(v[0][half], a[2 * half], a[1 + 2 * half]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_16816<false>(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
+        for (int n = 0; n < NT; ++n) mma_16816(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
     }
+}
+
+// A bf16 pair times the power of two f, as an fp16 pair.
+__device__ __forceinline__ uint32_t bf16_to_f16(uint32_t x, float f) {
+    const __half2 h = __floats2half2_rn(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f);
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // grid (splits, n_heads * row tiles, batch); a CTA's warps take the 16-token
@@ -145,6 +138,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
 
     // Q's B registers: row n = lane / 4 of each 8-row group, this lane's blocks
     uint32_t qf[NT][KW * 4];
+    float qk[NT][2];  // what a score of the lane's rows 2t, 2t + 1 is multiplied by
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const uint32_t r = row0 + 8 * n + g;
@@ -152,15 +146,39 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
         const uint32_t qt = in ? a.by_group.div(r) : 0, qh = h * a.group + (in ? r - qt * a.group : 0);
         const uint4 *qp = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
                                                           qh * a.q_stride_h + qt * a.q_stride_t);
+        uint4 u[KW];
 #pragma unroll
-        for (int j = 0; j < KW; ++j) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (in) u = __ldg(qp + t * KW + j);
-            // code_pair S holds channels (7 - S, 3 - S): low half channel 7 - S
-            qf[n][4 * j + 0] = __byte_perm(u.w, u.y, 0x7632);
-            qf[n][4 * j + 1] = __byte_perm(u.w, u.y, 0x5410);
-            qf[n][4 * j + 2] = __byte_perm(u.z, u.x, 0x7632);
-            qf[n][4 * j + 3] = __byte_perm(u.z, u.x, 0x5410);
+        for (int j = 0; j < KW; ++j) u[j] = in ? __ldg(qp + t * KW + j) : make_uint4(0, 0, 0, 0);
+        float back = a.qk_log2 * kCodeUnit;
+        if constexpr (BF16) {
+            uint32_t e = 0;  // the row's largest finite exponent
+#pragma unroll
+            for (int j = 0; j < KW; ++j) {
+                const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t lo = w[i] >> 7 & 0xffu, hi = w[i] >> 23 & 0xffu;
+                    e = max(e, max(lo == 0xffu ? 0u : lo, hi == 0xffu ? 0u : hi));
+                }
+            }
+            e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
+            e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
+            e = max(e, 27u);  // rows under 2^-100 count as 2^-100
+            const float f = __uint_as_float((264u - e) << 23);  // 2^(10 - (e - 127))
+            back *= __uint_as_float((e - 10u) << 23);           // 1 / f
+#pragma unroll
+            for (int j = 0; j < KW; ++j)
+                u[j] = make_uint4(bf16_to_f16(u[j].x, f), bf16_to_f16(u[j].y, f), bf16_to_f16(u[j].z, f),
+                                  bf16_to_f16(u[j].w, f));
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) qk[n][c] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + c));
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {  // decode_block's pair s: channels 7 - s, 3 - s
+            qf[n][4 * j + 0] = __byte_perm(u[j].w, u[j].y, 0x7632);
+            qf[n][4 * j + 1] = __byte_perm(u[j].w, u[j].y, 0x5410);
+            qf[n][4 * j + 2] = __byte_perm(u[j].z, u[j].x, 0x7632);
+            qf[n][4 * j + 3] = __byte_perm(u[j].z, u[j].x, 0x5410);
         }
     }
 
@@ -203,15 +221,13 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
         for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
-            const CodeWord c0 = code_word<BF16>(x.k[0][j]), c1 = code_word<BF16>(x.k[1][j]);
-            const uint32_t a0 = code_pair<BF16, 0>(c0), a1 = code_pair<BF16, 0>(c1);
-            const uint32_t a2 = code_pair<BF16, 1>(c0), a3 = code_pair<BF16, 1>(c1);
-            const uint32_t a4 = code_pair<BF16, 2>(c0), a5 = code_pair<BF16, 2>(c1);
-            const uint32_t a6 = code_pair<BF16, 3>(c0), a7 = code_pair<BF16, 3>(c1);
+            uint32_t k0[4], k1[4];
+            decode_block(x.k[0][j], k0);
+            decode_block(x.k[1][j], k1);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                mma_16816<BF16>(s[n], a0, a1, a2, a3, qf[n][4 * j], qf[n][4 * j + 1]);
-                mma_16816<BF16>(s[n], a4, a5, a6, a7, qf[n][4 * j + 2], qf[n][4 * j + 3]);
+                mma_16816(s[n], k0[0], k1[0], k0[1], k1[1], qf[n][4 * j], qf[n][4 * j + 1]);
+                mma_16816(s[n], k0[2], k1[2], k0[3], k1[3], qf[n][4 * j + 2], qf[n][4 * j + 3]);
             }
         }
 
@@ -219,12 +235,12 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
         float rvs[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const float kx = x.ks[r] * (a.qk_log2 * kCodeUnit<BF16>), lv = __log2f(x.vs[r]);
+            const float lv = __log2f(x.vs[r]);
             rvs[r] = __frcp_rn(x.vs[r]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                s[n][2 * r] = fmaf(s[n][2 * r], kx, lv);
-                s[n][2 * r + 1] = fmaf(s[n][2 * r + 1], kx, lv);
+                s[n][2 * r] = fmaf(s[n][2 * r], x.ks[r] * qk[n][0], lv);
+                s[n][2 * r + 1] = fmaf(s[n][2 * r + 1], x.ks[r] * qk[n][1], lv);
             }
         }
         if (tok + 16 > drafts || bad) {  // drafts, tokens past the end: whole warp
@@ -282,15 +298,15 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
                 p[n][r] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&hw));
             }
 
-        CodeWord c[4][VW];
+        TokenPair v[VW][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < VW; ++j)
 #pragma unroll
-            for (int j = 0; j < VW; ++j) c[i][j] = code_word<false>(x.v[i][j]);
-        pv_step<D, NT, 0>(c, p, o);
-        pv_step<D, NT, 1>(c, p, o);
-        pv_step<D, NT, 2>(c, p, o);
-        pv_step<D, NT, 3>(c, p, o);
+            for (int half = 0; half < 2; ++half) v[j][half] = pair_tokens(x.v[2 * half][j], x.v[2 * half + 1][j]);
+        pv_step<D, NT, 0>(v, p, o);
+        pv_step<D, NT, 1>(v, p, o);
+        pv_step<D, NT, 2>(v, p, o);
+        pv_step<D, NT, 3>(v, p, o);
     }
 
     // the warps' statistics and outputs, merged in warp order

@@ -57,7 +57,7 @@ __device__ __forceinline__ void paged_store(const PagedAttnArgs &a, uint32_t b, 
     const uint32_t t = a.by_group.div(r), qh = h * a.group + (r - t * a.group);
     const int64_t row = ((int64_t)b * a.n_heads * a.group + qh) * a.T + t;
     // a row that sees nothing has l = 0 (a NaN denominator stays NaN)
-    Elem<BF16 ? LQ_BF16 : LQ_F16>::store(a.out, row * D + d, l == 0.f ? 0.f : o * kCodeUnit<false> / l);
+    Elem<BF16 ? LQ_BF16 : LQ_F16>::store(a.out, row * D + d, l == 0.f ? 0.f : o * kCodeUnit / l);
     if (a.lse && d == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
