@@ -70,25 +70,30 @@ struct Tile {
     float ks[2], vs[2];
 };
 
+// Where a tile's rows are: the K words, V words and scales of its first token.
+struct TileAt {
+    const uint32_t *k, *v;
+    const float *ks, *vs;
+};
+
 template <int D>
-__device__ __forceinline__ void load_tile(const PagedAttnArgs &a, const uint32_t *kbase, const float *sbase, int64_t page,
-                                          uint32_t off, uint32_t g, uint32_t t, Tile<D> &x) {
-    constexpr int W = D / 8;
-    // the page's K rows of this head (kbase is the head's offset in page 0)
-    const int64_t side = (int64_t)a.n_heads << a.page_log2;
-    const int64_t row = 2 * side * page + off;
-    const uint32_t *kp = kbase + row * W;
-    const uint32_t *vp = kp + side * W;
-    const float *sp = sbase + row;
+__device__ __forceinline__ void load_k(const TileAt &at, uint32_t g, uint32_t t, Tile<D> &x) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) load_words<Tile<D>::KW>(at.k + (g + 8 * r) * (D / 8) + t * Tile<D>::KW, x.k[r]);
+}
+template <int D>
+__device__ __forceinline__ void load_scales(const TileAt &at, uint32_t g, Tile<D> &x) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        load_words<Tile<D>::KW>(kp + (g + 8 * r) * W + t * Tile<D>::KW, x.k[r]);
-        x.ks[r] = __ldg(sp + g + 8 * r);
-        x.vs[r] = __ldg(sp + side + g + 8 * r);
+        x.ks[r] = __ldg(at.ks + g + 8 * r);
+        x.vs[r] = __ldg(at.vs + g + 8 * r);
     }
+}
+template <int D>
+__device__ __forceinline__ void load_v(const TileAt &at, uint32_t g, uint32_t t, Tile<D> &x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        load_words<Tile<D>::VW>(vp + (2 * t + (i & 1) + 8 * (i >> 1)) * W + g * Tile<D>::VW, x.v[i]);
+        load_words<Tile<D>::VW>(at.v + (2 * t + (i & 1) + 8 * (i >> 1)) * (D / 8) + g * Tile<D>::VW, x.v[i]);
 }
 
 // v[block][half]: tokens 2t, 2t+1 (+ 8 half) of this lane's blocks
@@ -123,7 +128,7 @@ __device__ __forceinline__ uint32_t bf16_to_f16(uint32_t x, float f) {
 // grid (splits, n_heads * row tiles, batch); a CTA's warps take the 16-token
 // tiles of its chunk in turn.
 template <bool BF16, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int KW = D / 32, VW = D / 64, W = D / 8, MT = D / 16;
     constexpr int ROWS = 8 * NT;
     extern __shared__ __align__(16) float sm[];  // [warps][ROWS][D + 2]
@@ -131,9 +136,10 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t b = blockIdx.z, rt = blockIdx.y / a.n_heads, h = blockIdx.y - rt * a.n_heads;
     const uint32_t row0 = rt * ROWS;
-    const int64_t len = paged_len(a, b);
-    const int64_t first = (int64_t)blockIdx.x * a.chunk, last = min(first + a.chunk, len);
-    const int64_t drafts = len - a.T;  // position of draft 0
+    // positions fit 32 bits: a table is at most 2^20 pages of 2^8 tokens
+    const int len = (int)paged_len(a, b);
+    const int first = (int)(blockIdx.x * a.chunk), last = (int)min(first + a.chunk, (int64_t)len);
+    const int drafts = len - (int)a.T;  // position of draft 0
     if (len < a.lens[b] && (blockIdx.x | blockIdx.y | threadIdx.x) == 0) raise_flag(a.err, LQ_EF_PAGE);
 
     // Q's B registers: row n = lane / 4 of each 8-row group, this lane's blocks
@@ -196,25 +202,32 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
     const int32_t *table = a.table + b * a.table_stride;
     const uint32_t *kbase = a.codes + ((int64_t)h << a.page_log2) * W;
     const float *sbase = a.scales + ((int64_t)h << a.page_log2);
-    const uint32_t page_mask = (1u << a.page_log2) - 1;
+    const int64_t side = (int64_t)a.n_heads << a.page_log2;
+    const int page_mask = (1 << a.page_log2) - 1, n_pages = (int)a.n_pages;
+    constexpr int kStep = 16 * kWarps;
     // a table entry outside the pool is reported, and read as page 0 with its tokens masked
-    auto page_of = [&](int64_t tok) -> int64_t {
-        return tok < last ? (int64_t)__ldg(table + (tok >> a.page_log2)) : 0;
+    auto page_of = [&](int tok) { return tok < last ? __ldg(table + (tok >> a.page_log2)) : 0; };
+    auto usable = [&](int page) { return (uint32_t)page < (uint32_t)n_pages; };
+    auto locate = [&](int tok, int page) {
+        const int64_t row = 2 * side * (usable(page) ? page : 0) + (tok & page_mask);
+        const uint32_t *k = kbase + row * W;
+        return TileAt{k, k + side * W, sbase + row, sbase + row + side};
     };
-    auto usable = [&](int64_t page) { return page >= 0 && page < a.n_pages; };
 
-    int64_t tok = first + 16 * warp;
-    Tile<D> nx;
-    int64_t page_nx = page_of(tok);
-    if (tok < last) load_tile<D>(a, kbase, sbase, usable(page_nx) ? page_nx : 0, (uint32_t)tok & page_mask, g, t, nx);
-    int64_t page_nn = page_of(tok + 16 * kWarps);
-    for (; tok < last; tok += 16 * kWarps) {
-        const Tile<D> x = nx;
-        const bool bad = !usable(page_nx);
-        page_nx = page_nn;
-        const int64_t tn = tok + 16 * kWarps;
-        if (tn < last) load_tile<D>(a, kbase, sbase, usable(page_nx) ? page_nx : 0, (uint32_t)tn & page_mask, g, t, nx);
-        page_nn = page_of(tn + 16 * kWarps);
+    int page = page_of(first + 16 * warp), page_nx = page_of(first + 16 * warp + kStep);
+    Tile<D> x;
+    if (first + 16 * warp < last) {
+        const TileAt at = locate(first + 16 * warp, page);
+        load_k<D>(at, g, t, x);
+        load_scales<D>(at, g, x);
+        load_v<D>(at, g, t, x);
+    }
+    for (int tok = first + 16 * warp; tok < last; tok += kStep) {
+        // the next tile's words load into x as soon as this one's are decoded
+        const bool bad = !usable(page), more = tok + kStep < last;
+        const TileAt next = locate(tok + kStep, page_nx);
+        page = page_nx;
+        page_nx = page_of(tok + 2 * kStep);
 
         float s[NT][4];
 #pragma unroll
@@ -231,23 +244,26 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
             }
         }
 
+        if (more) load_k<D>(next, g, t, x);
+
         // x = s * ks + log2(vs), and 1 / vs for the denominator
         float rvs[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const float lv = __log2f(x.vs[r]);
-            rvs[r] = __frcp_rn(x.vs[r]);
+            const float lv = lg2(x.vs[r]);
+            rvs[r] = rcp(x.vs[r]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 s[n][2 * r] = fmaf(s[n][2 * r], x.ks[r] * qk[n][0], lv);
                 s[n][2 * r + 1] = fmaf(s[n][2 * r + 1], x.ks[r] * qk[n][1], lv);
             }
         }
+        if (more) load_scales<D>(next, g, x);
         if (tok + 16 > drafts || bad) {  // drafts, tokens past the end: whole warp
             if (bad && lane == 0) raise_flag(a.err, LQ_EF_PAGE);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int64_t p = tok + g + 8 * r;
+                const int p = tok + (int)g + 8 * r;
                 const bool past = p >= last || bad;
                 if (past) rvs[r] = 0.f;
 #pragma unroll
@@ -303,6 +319,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_kernel(const __grid_co
         for (int j = 0; j < VW; ++j)
 #pragma unroll
             for (int half = 0; half < 2; ++half) v[j][half] = pair_tokens(x.v[2 * half][j], x.v[2 * half + 1][j]);
+        if (more) load_v<D>(next, g, t, x);
         pv_step<D, NT, 0>(v, p, o);
         pv_step<D, NT, 1>(v, p, o);
         pv_step<D, NT, 2>(v, p, o);
