@@ -29,6 +29,7 @@ namespace lq {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int64_t kFewRows = 8;  // up to here this kernel, above lq_paged_attn_tc.cu
 
 __device__ __forceinline__ void mma_16816(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -117,12 +118,6 @@ __device__ __forceinline__ void pv_step(const TokenPair v[D / 64][2], const uint
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_16816(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
     }
-}
-
-// A bf16 pair times the power of two f, as an fp16 pair.
-__device__ __forceinline__ uint32_t bf16_to_f16(uint32_t x, float f) {
-    const __half2 h = __floats2half2_rn(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f);
-    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // grid (splits, n_heads * row tiles, batch); a CTA's warps take the 16-token
@@ -391,37 +386,36 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
     paged_store<BF16, D>(a, b, h, r, d, od, ld, mx);
 }
 
-template <bool BF16, int D, int NT>
-int launch_rows(const PagedAttnArgs &a, uint32_t batch, cudaStream_t st) {
-    const size_t smem = (size_t)kWarps * 8 * NT * (D + 2) * 4;
-    const uint32_t tiles = (uint32_t)ceil_div(a.rows, 8 * NT);
-    paged_attn_kernel<BF16, D, NT><<<dim3(a.splits, a.n_heads * tiles, batch), 32 * kWarps, smem, st>>>(a);
-    if (check_launch() != LQ_OK) return LQ_ERR_CUDA;
-    if (a.splits > 1) {
-        const uint32_t n = batch * a.n_heads * a.rows;
-        paged_combine_kernel<BF16, D><<<(unsigned)ceil_div(n, 128 / D), 128, 0, st>>>(a, n);
-    }
+template <bool BF16, int D>
+int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st) {
+    if (tile == 8)
+        paged_attn_kernel<BF16, D, 1><<<dim3(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, 8), batch), 32 * kWarps,
+                                        kWarps * 8 * (D + 2) * 4, st>>>(a);
+    const int status = tile == 8 ? check_launch() : launch_paged_tc(a, BF16, D, tile, batch, st);
+    if (status != LQ_OK || a.splits == 1) return status;
+    const uint32_t n = batch * a.n_heads * a.rows;
+    paged_combine_kernel<BF16, D><<<(unsigned)ceil_div(n, 128 / D), 128, 0, st>>>(a, n);
     return check_launch();
 }
 
-template <bool BF16, int D>
-int launch_dim(const PagedAttnArgs &a, uint32_t batch, cudaStream_t st) {
-    return a.rows <= 8 ? launch_rows<BF16, D, 1>(a, batch, st) : launch_rows<BF16, D, 2>(a, batch, st);
-}
-
-// Tokens of one split: enough CTAs for about four rounds of the GPU, chunks
-// of at least 64 tokens (a tile for each warp).
+// Rows of a CTA and tokens of a split: enough CTAs for about four rounds of
+// the GPU, chunks of a tile of tokens at least.
 struct Plan {
+    int tile;
     int64_t chunk;
     uint32_t splits;
 };
 
 Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
-    const int64_t tiles = ceil_div(rows, rows <= 8 ? 8 : 16);
-    const int64_t units = batch * n_heads * tiles;  // CTAs without a split
-    const int64_t want = ceil_div((int64_t)148 * 16, units);
-    int64_t chunk = ceil_div(ceil_div(max_len < 1 ? 1 : max_len, want), 64) * 64;
-    return Plan{chunk, (uint32_t)ceil_div(max_len < 1 ? 1 : max_len, chunk)};
+    Plan p;
+    p.tile = rows <= kFewRows ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    const int64_t least = p.tile == 8 ? 64 : 128;
+    const int64_t units = batch * n_heads * ceil_div(rows, p.tile);  // CTAs without a split
+    const int64_t want = ceil_div((int64_t)148 * (p.tile == 8 ? 16 : p.tile == 16 ? 12 : 8), units);
+    const int64_t tokens = max_len < 1 ? 1 : max_len;
+    p.chunk = ceil_div(ceil_div(tokens, want), least) * least;
+    p.splits = (uint32_t)ceil_div(tokens, p.chunk);
+    return p;
 }
 
 }  // namespace
@@ -496,6 +490,7 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
     a.err = err;
     cudaStream_t st = as_stream(stream);
     const uint32_t B = (uint32_t)batch;
-    if (q_dtype == LQ_BF16) return head_dim == 128 ? launch_dim<true, 128>(a, B, st) : launch_dim<true, 64>(a, B, st);
-    return head_dim == 128 ? launch_dim<false, 128>(a, B, st) : launch_dim<false, 64>(a, B, st);
+    if (q_dtype == LQ_BF16)
+        return head_dim == 128 ? launch_dim<true, 128>(a, p.tile, B, st) : launch_dim<true, 64>(a, p.tile, B, st);
+    return head_dim == 128 ? launch_dim<false, 128>(a, p.tile, B, st) : launch_dim<false, 64>(a, p.tile, B, st);
 }

@@ -88,4 +88,14 @@ __device__ __forceinline__ void paged_emit(const PagedAttnArgs &a, uint32_t b, u
     }
 }
 
+// A bf16 pair times the power of two f, as an fp16 pair.
+__device__ __forceinline__ uint32_t bf16_to_f16(uint32_t x, float f) {
+    const __half2 h = __floats2half2_rn(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// The tensor-core kernel for many rows (lq_paged_attn_tc.cu): `tile` rows a
+// CTA, 16, 32 or 64; a.chunk a multiple of 128.
+int launch_paged_tc(const PagedAttnArgs &a, bool bf16, int head_dim, int tile, uint32_t batch, cudaStream_t st);
+
 }  // namespace lq

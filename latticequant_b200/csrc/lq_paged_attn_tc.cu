@@ -1,0 +1,456 @@
+// lq_paged_attn_tc.cu -- attention over the pages of an E8 cache on the
+// 5th-generation tensor cores, for many query rows (trees, prompt chunks).
+//
+// The same mathematics as lq_paged_attn.cu, in the same transposed form: a
+// CTA takes 128 tokens at a time and up to N query rows of one KV head,
+//   S^T [128 tokens x N] = K [128 x D] Q^T      (tcgen05.mma, into TMEM)
+//   x = S^T * ks * c + log2(vs),  w = 2^(x - M),  l += w / vs
+//   O^T [D x N] += V^T [D x 128] W^T [128 x N]  (tcgen05.mma, stays in TMEM)
+// Tokens are the MMA's 128 rows, so no row is padding however few queries
+// there are; a thread owns one token (a TMEM lane) and half of the N columns.
+//
+// The 256 threads decode a tile's code words straight into the swizzled
+// shared-memory layout that both MMAs read (a decoded block of 8 channels is one 16-byte
+// chunk; V^T is read from the same token-major layout as an MN-major
+// operand).  The order of a tile keeps the tensor cores busy beside them:
+//   decode K | S starts | decode V | wait S, weights | O starts | decode next K ..
+// and two or three CTAs share an SM.  What bounds it is instruction issue:
+// the decode (about 20 instructions a block) and six a score.
+//
+// M is a reference per row, moved only when an x exceeds it by kRefSlack,
+// which a block-wide vote finds; O is then rescaled in TMEM.
+//
+// Every wait is bounded (LQ_EF_TIMEOUT after about a second; the results are
+// then wrong, and later waits return at once).
+#include "lq_paged_attn.cuh"
+
+namespace lq {
+namespace {
+
+constexpr int kTok = 128;       // tokens of a tile
+constexpr int kThreads = 256;
+constexpr int kHalfBytes = kTok * 128;  // a tile's 64 channels in fp16, 128-byte rows
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void store16(uint32_t addr, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                 : "memory");
+}
+
+// Matrix descriptor of a 128-byte-swizzled operand: lead and stride in bytes.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride) {
+    return (uint64_t)(addr >> 4 & 0x3fffu) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 |
+           2ull << 61;
+}
+
+// Instruction descriptor: fp16 operands, fp32 accumulator, M = 128.
+template <int N>
+constexpr uint32_t kShape = 1u << 4 | (uint32_t)(N >> 3) << 17 | (128u >> 4) << 24;
+constexpr uint32_t kTransposeA = 1u << 15;
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(shape), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_done(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Waits for the barrier's phase, at most about a second; false then.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t phase) {
+    const long long start = clock64();
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+            : "=r"(ok)
+            : "r"(bar), "r"(phase)
+            : "memory");
+        if (ok) return true;
+        if (clock64() - start > 2000000000ll) return false;
+    }
+}
+
+// C consecutive TMEM columns of the warp's 32 lanes.
+template <int C>
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[C]) {
+    static_assert(C % 8 == 0);
+#pragma unroll
+    for (int i = 0; i < C; i += 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]), "=f"(v[i + 4]), "=f"(v[i + 5]),
+                       "=f"(v[i + 6]), "=f"(v[i + 7])
+                     : "r"(addr + i));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < C; ++i) asm volatile("" : "+f"(v[i]));  // no use of v moves above the wait
+}
+template <int C>
+__device__ __forceinline__ void tmem_store(uint32_t addr, const float (&v)[C]) {
+#pragma unroll
+    for (int i = 0; i < C; i += 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr + i),
+                     "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]),
+                     "f"(v[i + 6]), "f"(v[i + 7])
+                     : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Generic writes to shared memory become visible to the tensor cores.
+__device__ __forceinline__ void publish_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Shared memory after the 1024-byte aligned operands.
+template <int N>
+struct Small {
+    uint64_t bar_s, bar_o;
+    uint32_t tmem, exponent;
+    alignas(16) float m[N];
+    float f[N], red[8][N / 2];
+};
+
+template <int D, int N>
+constexpr size_t smem_bytes() {
+    return 1024 + 2 * (size_t)(D / 64) * kHalfBytes + (size_t)N * D * 2 + (size_t)N * kTok * 2 + sizeof(Small<N>);
+}
+
+// The lane order of a decoded block: position p holds channel kChannel >> 4p & 15.
+constexpr uint32_t kChannel = 0x04152637u;
+
+template <bool BF16, int D, int N>
+__global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
+    paged_attn_tc_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int W = D / 8, H = D / 64, C = N / 2;  // words of a row, 64-channel halves, columns of a thread
+    constexpr int RPT = D / 64;                      // token rows a thread decodes (four words of each)
+    constexpr uint32_t kCols = N <= 16 ? 32 : 2 * N; // TMEM: S^T and O^T
+    extern __shared__ char raw[];
+    char *buf = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    // V first: at D = 64 the O MMA's upper 64 rows read past it, into K (and are not used)
+    const uint32_t sv = smem_u32(buf), sk = sv + H * kHalfBytes, sq = sk + H * kHalfBytes, sp = sq + N * D * 2;
+    Small<N> &sm = *reinterpret_cast<Small<N> *>(buf + 2 * H * kHalfBytes + N * D * 2 + N * kTok * 2);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t b = blockIdx.z, rt = blockIdx.y / a.n_heads, h = blockIdx.y - rt * a.n_heads;
+    const uint32_t row0 = rt * N;
+    const int len = (int)paged_len(a, b);
+    const int first = (int)(blockIdx.x * a.chunk), last = (int)min(first + a.chunk, (int64_t)len);
+    const int drafts = len - (int)a.T;
+    if (len < a.lens[b] && (blockIdx.x | blockIdx.y | tid) == 0) raise_flag(a.err, LQ_EF_PAGE);
+    const int live = (int)min((uint32_t)N, a.rows - row0);
+    if (first >= last) {  // nothing to read; without a split the rows are still written
+        if (a.splits == 1)
+            for (int e = tid; e < live * D; e += kThreads)
+                paged_store<BF16, D>(a, b, h, row0 + e / D, e % D, 0.f, 0.f, kNoRef);
+        return;
+    }
+
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
+                     "r"(kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 0) {
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&sm.bar_s)) : "memory");
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&sm.bar_o)) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        sm.exponent = 27;
+    }
+    for (int n = tid; n < N; n += kThreads) sm.m[n] = kNoRef;
+
+    // ---- Q: fp16 rows in the decoded blocks' channel order; rows past the last are zero
+    constexpr int kChunks = N * W;  // 16-byte chunks
+    constexpr int kQ = (kChunks + kThreads - 1) / kThreads;
+    uint4 q[kQ];
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+        const int e = tid + i * kThreads, n = e / W, c = e % W;
+        q[i] = make_uint4(0, 0, 0, 0);
+        if (e < kChunks && n < live) {
+            const uint32_t r = row0 + n, qt = a.by_group.div(r), qh = h * a.group + (r - qt * a.group);
+            q[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
+                                                         qh * a.q_stride_h + qt * a.q_stride_t) + c);
+        }
+    }
+    float qk = a.qk_log2 * kCodeUnit;
+    if constexpr (BF16) {  // a power of two for all rows puts the largest finite value in [2^10, 2^11)
+        uint32_t e = 27;   // (at least 2^-100)
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
+            const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t lo = w[k] >> 7 & 0xffu, hi = w[k] >> 23 & 0xffu;
+                e = max(e, max(lo == 0xffu ? 0u : lo, hi == 0xffu ? 0u : hi));
+            }
+        }
+        e = __reduce_max_sync(0xffffffffu, e);
+        __syncthreads();
+        if (lane == 0) atomicMax(&sm.exponent, e);
+        __syncthreads();
+        e = sm.exponent;
+        const float f = __uint_as_float((264u - e) << 23);
+        qk *= __uint_as_float((e - 10u) << 23);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            q[i] = make_uint4(bf16_to_f16(q[i].x, f), bf16_to_f16(q[i].y, f), bf16_to_f16(q[i].z, f),
+                              bf16_to_f16(q[i].w, f));
+    }
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+        const int e = tid + i * kThreads, n = e / W, c = e % W;
+        if (e >= kChunks) break;
+        // pairs (7, 3), (6, 2), (5, 1), (4, 0)
+        const uint32_t v[4] = {__byte_perm(q[i].w, q[i].y, 0x7632), __byte_perm(q[i].w, q[i].y, 0x5410),
+                               __byte_perm(q[i].z, q[i].x, 0x7632), __byte_perm(q[i].z, q[i].x, 0x5410)};
+        store16(sq + (c >> 3) * (N * 128) + n * 128 + (((c & 7) ^ (n & 7)) << 4), v);
+    }
+
+    // ---- what this thread reads of a tile: RPT rows of four words each of K and V, the scales of its token
+    constexpr int kPerRow = W / 4;  // threads of a row
+    const int part = tid % kPerRow, drow = tid / kPerRow;
+    constexpr int kRowStep = kThreads / kPerRow;
+    const int tl = (warp & 3) * 32 + lane;  // the token (TMEM lane) whose scores it handles
+    const int col0 = (warp >> 2) * C;
+    const int32_t *table = a.table + b * a.table_stride;
+    const int64_t side = (int64_t)a.n_heads << a.page_log2;
+    const uint32_t *kbase = a.codes + ((int64_t)h << a.page_log2) * W + part * 4;
+    const float *sbase = a.scales + ((int64_t)h << a.page_log2);
+    const int page_mask = (1 << a.page_log2) - 1;
+    bool bad = false;  // a table entry outside the pool: reported, read as page 0, masked
+    auto row_of = [&](int tok) -> int64_t {
+        if (tok >= last) return 0;
+        const int page = __ldg(table + (tok >> a.page_log2));
+        const bool ok = (uint32_t)page < (uint32_t)a.n_pages;
+        return 2 * side * (ok ? page : 0) + (tok & page_mask);
+    };
+    uint4 kw[RPT], vw[RPT];
+    float ks, vs;
+    auto fetch_k = [&](int t0) {
+#pragma unroll
+        for (int r = 0; r < RPT; ++r)
+            kw[r] = __ldg(reinterpret_cast<const uint4 *>(kbase + row_of(t0 + drow + r * kRowStep) * W));
+    };
+    auto fetch_v = [&](int t0) {
+#pragma unroll
+        for (int r = 0; r < RPT; ++r)
+            vw[r] = __ldg(reinterpret_cast<const uint4 *>(kbase + (row_of(t0 + drow + r * kRowStep) + side) * W));
+    };
+    auto fetch_scales = [&](int t0) {
+        const int tok = t0 + tl;
+        const int page = tok < last ? __ldg(table + (tok >> a.page_log2)) : 0;
+        bad = (uint32_t)page >= (uint32_t)a.n_pages;
+        const int64_t row = 2 * side * (bad ? 0 : page) + (tok & page_mask);
+        ks = __ldg(sbase + row);
+        vs = __ldg(sbase + row + side);
+    };
+    // decoded rows into an operand: at D = 128 the two 64-channel halves fall on the same banks, so the
+    // threads of the upper one take their words in the order 2, 3, 0, 1
+    const bool upper = D == 128 && part >= 2;
+    auto put = [&](uint32_t dst, const uint4 (&w)[RPT]) {
+#pragma unroll
+        for (int r = 0; r < RPT; ++r) {
+            const int row = drow + r * kRowStep;
+            const uint32_t v[4] = {upper ? w[r].z : w[r].x, upper ? w[r].w : w[r].y, upper ? w[r].x : w[r].z,
+                                   upper ? w[r].y : w[r].w};
+            const uint32_t line = dst + (D == 128 ? (part >> 1) * kHalfBytes : 0) + row * 128;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t pair[4];
+                decode_block(v[j], pair);
+                const uint32_t chunk = ((part & 1) * 4 + j) ^ (upper ? 2u : 0u);
+                store16(line + ((chunk ^ (row & 7)) << 4), pair);
+            }
+        }
+    };
+
+    fetch_k(first);
+    fetch_v(first);
+    fetch_scales(first);
+    publish_smem();
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t ts = sm.tmem, to = ts + N, my_lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t bar_s = smem_u32(&sm.bar_s), bar_o = smem_u32(&sm.bar_o);
+    const uint64_t dk = operand(sk, 16, 1024), dq = operand(sq, 16, 1024), dp = operand(sp, 16, 1024),
+                   dv = operand(sv, kHalfBytes, 1024);
+
+    float l[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) l[c] = 0.f;
+    bool alive = true;
+    uint32_t phase = 0;  // of both barriers, per tile
+    for (int t0 = first; t0 < last; t0 += kTok, phase ^= 1) {
+        const bool more = t0 + kTok < last;
+        put(sk, kw);
+        if (more) fetch_k(t0 + kTok);
+        publish_smem();
+        tmem_fence_before();
+        __syncthreads();
+        if (tid == 0) {
+            tmem_fence_after();
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t in = (k & 3) * 2;  // 32 bytes on within the swizzled rows
+                mma(ts, dk + (k >> 2) * (kHalfBytes >> 4) + in, dq + (k >> 2) * (N * 128 >> 4) + in, kShape<N>, k > 0);
+            }
+            mma_done(bar_s);
+        }
+        if (t0 > first) alive = alive && wait_for(bar_o, phase ^ 1);  // V's and W's buffers are free
+        put(sv, vw);
+        if (more) fetch_v(t0 + kTok);
+
+        alive = alive && wait_for(bar_s, phase);
+        tmem_fence_after();
+        const int tok = t0 + tl;
+        const bool past = tok >= last || bad;
+        if (bad && tok < last) raise_flag(a.err, LQ_EF_PAGE);
+        const float kx = ks * qk, lv = lg2(vs), rvs = past ? 0.f : rcp(vs);
+        if (more) fetch_scales(t0 + kTok);
+        uint32_t hidden = past ? 0xffffffffu : 0u;  // columns that do not see the token
+        if (tok >= drafts && !past)
+#pragma unroll 1
+            for (uint32_t c = 0; c < C && row0 + col0 + c < a.rows; ++c)
+                hidden |= (uint32_t)!paged_sees(a, b, a.by_group.div(row0 + col0 + c), tok - drafts) << c;
+        float x[C];
+        auto scores = [&]() {
+            tmem_load<C>(ts + my_lanes + col0, x);
+#pragma unroll
+            for (int c = 0; c < C; ++c) x[c] = fmaf(x[c], kx, lv);
+            if (__any_sync(0xffffffffu, hidden != 0)) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) x[c] = hidden >> c & 1 ? -INFINITY : x[c];
+            }
+        };
+        auto less_reference = [&]() {
+            bool grow = false;
+#pragma unroll
+            for (int c = 0; c < C; c += 4) {
+                const float4 m = *reinterpret_cast<const float4 *>(sm.m + col0 + c);
+                x[c] -= m.x;
+                x[c + 1] -= m.y;
+                x[c + 2] -= m.z;
+                x[c + 3] -= m.w;
+                grow |= fmaxf(fmaxf(x[c], x[c + 1]), fmaxf(x[c + 2], x[c + 3])) > kRefSlack;
+            }
+            return grow;
+        };
+        scores();
+        if (__syncthreads_or(less_reference())) {
+            // the tile's column maxima move the references; l and O follow
+            scores();
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float top = x[c];
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if (lane == 0) sm.red[warp][c] = top;
+            }
+            __syncthreads();
+            for (int n = tid; n < N; n += kThreads) {
+                const int g = n / C, c = n % C;
+                const float top = fmaxf(fmaxf(sm.red[4 * g][c], sm.red[4 * g + 1][c]),
+                                        fmaxf(sm.red[4 * g + 2][c], sm.red[4 * g + 3][c]));
+                const float next = fmaxf(sm.m[n], top - kRefBelow);
+                sm.f[n] = ex2(sm.m[n] - next);
+                sm.m[n] = next;
+            }
+            __syncthreads();
+            less_reference();
+#pragma unroll
+            for (int c = 0; c < C; ++c) l[c] *= sm.f[col0 + c];
+            if (t0 > first) {  // this warp's lanes (channels) and columns of O; its MMAs are done
+                float o[C];
+                tmem_load<C>(to + my_lanes + col0, o);
+#pragma unroll
+                for (int c = 0; c < C; ++c) o[c] *= sm.f[col0 + c];
+                tmem_store<C>(to + my_lanes + col0, o);
+            }
+        }
+        // weights: column c of this token, K-major rows of 64 tokens
+        const uint32_t at = sp + (tl >> 6) * (N * 128) + (tl & 7) * 2;
+        const uint32_t chunk = tl >> 3 & 7;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int n = col0 + c;
+            const float w = ex2(x[c]);
+            l[c] = fmaf(w, rvs, l[c]);
+            const __half hw = __float2half_rn(w);
+            asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + n * 128 + ((chunk ^ (n & 7)) << 4)),
+                         "h"(*reinterpret_cast<const uint16_t *>(&hw))
+                         : "memory");
+        }
+        publish_smem();
+        tmem_fence_before();
+        __syncthreads();
+        if (tid == 0) {
+            tmem_fence_after();
+#pragma unroll
+            for (int k = 0; k < kTok / 16; ++k)
+                mma(to, dv + k * (2048 >> 4), dp + (k >> 2) * (N * 128 >> 4) + (k & 3) * 2, kShape<N> | kTransposeA,
+                    t0 > first || k > 0);
+            mma_done(bar_o);
+        }
+    }
+    alive = alive && wait_for(bar_o, phase ^ 1);
+    tmem_fence_after();
+    if (!alive) raise_flag(a.err, LQ_EF_TIMEOUT);
+
+    // denominators over the 128 tokens, then O: a lane is a channel
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
+        if (lane == 0) sm.red[warp][c] = l[c];
+    }
+    float o[C];
+    tmem_load<C>(to + my_lanes + col0, o);
+    // through shared memory (the operands are done with) to rows of channels
+    float *rows = reinterpret_cast<float *>(buf);
+    const int d = (tl & ~7) + (int)(kChannel >> (4 * (tl & 7)) & 15u);
+    if (D == 128 || tl < 64)
+#pragma unroll
+        for (int c = 0; c < C; ++c) rows[(col0 + c) * D + d] = o[c];
+    __syncthreads();
+    for (int e = tid; e < live * D; e += kThreads) {
+        const int n = e / D, g = n / C, c = n % C;
+        const float den = (sm.red[4 * g][c] + sm.red[4 * g + 1][c]) + (sm.red[4 * g + 2][c] + sm.red[4 * g + 3][c]);
+        paged_emit<BF16, D>(a, b, h, row0 + n, e % D, blockIdx.x, rows[e], den, sm.m[n]);
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 0)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(ts), "r"(kCols) : "memory");
+}
+
+template <bool BF16, int D, int N>
+int launch_n(const PagedAttnArgs &a, uint32_t batch, cudaStream_t st) {
+    constexpr size_t smem = smem_bytes<D, N>();
+    if (cudaFuncSetAttribute(paged_attn_tc_kernel<BF16, D, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+        cudaSuccess)
+        return LQ_ERR_CUDA;
+    paged_attn_tc_kernel<BF16, D, N>
+        <<<dim3(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, N), batch), kThreads, smem, st>>>(a);
+    return check_launch();
+}
+
+template <bool BF16, int D>
+int launch_d(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st) {
+    if (tile == 16) return launch_n<BF16, D, 16>(a, batch, st);
+    if (tile == 32) return launch_n<BF16, D, 32>(a, batch, st);
+    return launch_n<BF16, D, 64>(a, batch, st);
+}
+
+}  // namespace
+
+int launch_paged_tc(const PagedAttnArgs &a, bool bf16, int head_dim, int tile, uint32_t batch, cudaStream_t st) {
+    if (bf16) return head_dim == 128 ? launch_d<true, 128>(a, tile, batch, st) : launch_d<true, 64>(a, tile, batch, st);
+    return head_dim == 128 ? launch_d<false, 128>(a, tile, batch, st) : launch_d<false, 64>(a, tile, batch, st);
+}
+
+}  // namespace lq
