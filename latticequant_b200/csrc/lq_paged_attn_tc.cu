@@ -5,17 +5,18 @@
 // CTA takes 128 tokens at a time and up to N query rows of one KV head,
 //   S^T [128 tokens x N] = K [128 x D] Q^T      (tcgen05.mma, into TMEM)
 //   x = S^T * ks * c + log2(vs),  w = 2^(x - M),  l += w / vs
-//   O^T [D x N] += V^T [D x 128] W^T [128 x N]  (tcgen05.mma, stays in TMEM)
+//   O^T [D x N] += V^T [D x 128] W [128 x N]    (tcgen05.mma, stays in TMEM)
 // Tokens are the MMA's 128 rows, so no row is padding however few queries
 // there are; a thread owns one token (a TMEM lane) and half of the N columns.
 //
-// The 256 threads decode a tile's code words straight into the swizzled
-// shared-memory layout that both MMAs read (a decoded block of 8 channels is one 16-byte
-// chunk; V^T is read from the same token-major layout as an MN-major
-// operand).  The order of a tile keeps the tensor cores busy beside them:
-//   decode K | S starts | decode V | wait S, weights | O starts | decode next K ..
-// and two or three CTAs share an SM.  What bounds it is instruction issue:
-// the decode (about 20 instructions a block) and six a score.
+// The threads decode a tile's code words straight into the swizzled
+// shared-memory layout that both MMAs read (a decoded block of 8 channels is
+// one 16-byte chunk; V^T is read from the same token-major layout as an
+// MN-major operand, and so are the weights, a row of N per token).  The tensor cores run beside them, one tile apart:
+//   decode K of tile j+1 | decode V of tile j | scores of j, vote | S of j+1
+//   starts | weights of j | O of j starts | ..
+// with two barriers a tile.  What bounds it is instruction issue: the decode
+// (about 20 instructions a block) and four a score.
 //
 // M is a reference per row, moved only when an x exceeds it by kRefSlack,
 // which a block-wide vote finds; O is then rescaled in TMEM.
@@ -28,8 +29,7 @@ namespace lq {
 namespace {
 
 constexpr int kTok = 128;       // tokens of a tile
-constexpr int kThreads = 256;
-constexpr int kHalfBytes = kTok * 128;  // a tile's 64 channels in fp16, 128-byte rows
+constexpr int kHalfBytes = kTok * 128;  // 64 channels (or weights) of a tile's tokens in fp16, 128-byte rows
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -47,7 +47,7 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32
 // Instruction descriptor: fp16 operands, fp32 accumulator, M = 128.
 template <int N>
 constexpr uint32_t kShape = 1u << 4 | (uint32_t)(N >> 3) << 17 | (128u >> 4) << 24;
-constexpr uint32_t kTransposeA = 1u << 15;
+constexpr uint32_t kTransposeA = 1u << 15, kTransposeB = 1u << 16;
 
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool accumulate) {
     asm volatile(
@@ -109,29 +109,36 @@ template <int N>
 struct Small {
     uint64_t bar_s, bar_o;
     uint32_t tmem, exponent;
-    alignas(16) float m[N];
-    float f[N], red[8][N / 2];
+    alignas(16) float minus_m[N];
+    float f[N], red[4][N];
+    int pages[4][8];  // of four tiles; -1: outside the pool
 };
 
 template <int D, int N>
 constexpr size_t smem_bytes() {
-    return 1024 + 2 * (size_t)(D / 64) * kHalfBytes + (size_t)N * D * 2 + (size_t)N * kTok * 2 + sizeof(Small<N>);
+    return 1024 + 2 * (size_t)(D / 64) * kHalfBytes + (size_t)N * D * 2 + (size_t)(N + 63) / 64 * kHalfBytes + sizeof(Small<N>);
 }
 
 // The lane order of a decoded block: position p holds channel kChannel >> 4p & 15.
 constexpr uint32_t kChannel = 0x04152637u;
 
+template <int N>
+constexpr int kThreads = N <= 64 ? 256 : 512;
+
 template <bool BF16, int D, int N>
-__global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads<N>, N <= 16 ? 3 : N <= 64 ? 2 : 1)
     paged_attn_tc_kernel(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int W = D / 8, H = D / 64, C = N / 2;  // words of a row, 64-channel halves, columns of a thread
-    constexpr int RPT = D / 64;                      // token rows a thread decodes (four words of each)
-    constexpr uint32_t kCols = N <= 16 ? 32 : 2 * N; // TMEM: S^T and O^T
+    constexpr int kThreads = lq::kThreads<N>;
+    constexpr int W = D / 8, H = D / 64;              // words of a row, 64-channel halves
+    constexpr int C = N * 128 / kThreads;             // columns of a thread
+    constexpr int RPT = kTok * (W / 4) / kThreads;    // token rows a thread decodes, four words of each
+    constexpr uint32_t kCols = N <= 16 ? 64 : 4 * N;  // TMEM: S^T twice and O^T
+    static_assert(RPT >= 1 && kCols <= 512);
     extern __shared__ char raw[];
     char *buf = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     // V first: at D = 64 the O MMA's upper 64 rows read past it, into K (and are not used)
     const uint32_t sv = smem_u32(buf), sk = sv + H * kHalfBytes, sq = sk + H * kHalfBytes, sp = sq + N * D * 2;
-    Small<N> &sm = *reinterpret_cast<Small<N> *>(buf + 2 * H * kHalfBytes + N * D * 2 + N * kTok * 2);
+    Small<N> &sm = *reinterpret_cast<Small<N> *>(buf + 2 * H * kHalfBytes + N * D * 2 + (N + 63) / 64 * kHalfBytes);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t b = blockIdx.z, rt = blockIdx.y / a.n_heads, h = blockIdx.y - rt * a.n_heads;
@@ -160,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sm.exponent = 27;
     }
-    for (int n = tid; n < N; n += kThreads) sm.m[n] = kNoRef;
+    for (int n = tid; n < N; n += kThreads) sm.minus_m[n] = -kNoRef;
 
     // ---- Q: fp16 rows in the decoded blocks' channel order; rows past the last are zero
     constexpr int kChunks = N * W;  // 16-byte chunks
@@ -212,8 +219,8 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
 
     // ---- what this thread reads of a tile: RPT rows of four words each of K and V, the scales of its token
     constexpr int kPerRow = W / 4;  // threads of a row
-    const int part = tid % kPerRow, drow = tid / kPerRow;
     constexpr int kRowStep = kThreads / kPerRow;
+    const int part = tid % kPerRow, drow = tid / kPerRow;
     const int tl = (warp & 3) * 32 + lane;  // the token (TMEM lane) whose scores it handles
     const int col0 = (warp >> 2) * C;
     const int32_t *table = a.table + b * a.table_stride;
@@ -221,95 +228,117 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
     const uint32_t *kbase = a.codes + ((int64_t)h << a.page_log2) * W + part * 4;
     const float *sbase = a.scales + ((int64_t)h << a.page_log2);
     const int page_mask = (1 << a.page_log2) - 1;
-    bool bad = false;  // a table entry outside the pool: reported, read as page 0, masked
-    auto row_of = [&](int tok) -> int64_t {
-        if (tok >= last) return 0;
-        const int page = __ldg(table + (tok >> a.page_log2));
-        const bool ok = (uint32_t)page < (uint32_t)a.n_pages;
-        return 2 * side * (ok ? page : 0) + (tok & page_mask);
+    // Entry i of a tile's pages (0 where it has none); kept in the ring as -1 where it lies outside the
+    // pool: reported, read as page 0, its tokens masked.
+    auto page_entry = [&](int t0, int i) {
+        const int tok = ((t0 >> a.page_log2) + i) << a.page_log2;
+        return max(tok, t0) < min(t0 + kTok, last) ? __ldg(table + (tok >> a.page_log2)) : 0;
+    };
+    auto keep_entry = [&](int t0, int i, int page) {
+        if ((uint32_t)page >= (uint32_t)a.n_pages) {
+            raise_flag(a.err, LQ_EF_PAGE);
+            page = -1;
+        }
+        sm.pages[t0 >> 7 & 3][i] = page;
+    };
+    auto page_of = [&](int t0, int i) {  // of token i of the tile at t0
+        return sm.pages[t0 >> 7 & 3][(((t0 & page_mask) + i) >> a.page_log2) & 7];
+    };
+    auto row_of = [&](int t0, int i) {
+        return 2 * side * max(page_of(t0, i), 0) + ((t0 + i) & page_mask);
     };
     uint4 kw[RPT], vw[RPT];
     float ks, vs;
+    bool bad;
     auto fetch_k = [&](int t0) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r)
-            kw[r] = __ldg(reinterpret_cast<const uint4 *>(kbase + row_of(t0 + drow + r * kRowStep) * W));
+            kw[r] = __ldg(reinterpret_cast<const uint4 *>(kbase + row_of(t0, drow + r * kRowStep) * W));
     };
     auto fetch_v = [&](int t0) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r)
-            vw[r] = __ldg(reinterpret_cast<const uint4 *>(kbase + (row_of(t0 + drow + r * kRowStep) + side) * W));
+            vw[r] = __ldg(reinterpret_cast<const uint4 *>(kbase + (row_of(t0, drow + r * kRowStep) + side) * W));
     };
     auto fetch_scales = [&](int t0) {
-        const int tok = t0 + tl;
-        const int page = tok < last ? __ldg(table + (tok >> a.page_log2)) : 0;
-        bad = (uint32_t)page >= (uint32_t)a.n_pages;
-        const int64_t row = 2 * side * (bad ? 0 : page) + (tok & page_mask);
+        const int64_t row = row_of(t0, tl);
+        bad = page_of(t0, tl) < 0;
         ks = __ldg(sbase + row);
         vs = __ldg(sbase + row + side);
     };
-    // decoded rows into an operand: at D = 128 the two 64-channel halves fall on the same banks, so the
-    // threads of the upper one take their words in the order 2, 3, 0, 1
+    // Decoded rows into an operand.  At D = 128 the two 64-channel halves fall on the same banks, so the
+    // threads of the upper one take their words in the order 2, 3, 0, 1.
     const bool upper = D == 128 && part >= 2;
+    uint32_t chunk_at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        chunk_at[j] = (D == 128 ? (part >> 1) * kHalfBytes : 0) + drow * 128 +
+                      (((((part & 1) * 4 + j) ^ (upper ? 2 : 0)) ^ (drow & 7)) << 4);
     auto put = [&](uint32_t dst, const uint4 (&w)[RPT]) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
-            const int row = drow + r * kRowStep;
             const uint32_t v[4] = {upper ? w[r].z : w[r].x, upper ? w[r].w : w[r].y, upper ? w[r].x : w[r].z,
                                    upper ? w[r].y : w[r].w};
-            const uint32_t line = dst + (D == 128 ? (part >> 1) * kHalfBytes : 0) + row * 128;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t pair[4];
                 decode_block(v[j], pair);
-                const uint32_t chunk = ((part & 1) * 4 + j) ^ (upper ? 2u : 0u);
-                store16(line + ((chunk ^ (row & 7)) << 4), pair);
+                store16(dst + chunk_at[j] + r * (kRowStep * 128), pair);
             }
         }
     };
+    static_assert(kRowStep % 8 == 0);  // the rows of a thread share their swizzle
 
+    if (tid < 24) keep_entry(first + tid / 8 * kTok, tid % 8, page_entry(first + tid / 8 * kTok, tid % 8));
+    int entry = tid < 8 ? page_entry(first + 3 * kTok, tid) : 0;  // on its way to the ring
+    __syncthreads();
     fetch_k(first);
     fetch_v(first);
     fetch_scales(first);
+    put(sk, kw);
+    if (first + kTok < last) fetch_k(first + kTok);
     publish_smem();
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t ts = sm.tmem, to = ts + N, my_lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = sm.tmem, to = ts + 2 * N, my_lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t bar_s = smem_u32(&sm.bar_s), bar_o = smem_u32(&sm.bar_o);
-    const uint64_t dk = operand(sk, 16, 1024), dq = operand(sq, 16, 1024), dp = operand(sp, 16, 1024),
+    const uint64_t dk = operand(sk, 16, 1024), dq = operand(sq, 16, 1024), dp = operand(sp, kHalfBytes, 1024),
                    dv = operand(sv, kHalfBytes, 1024);
-
-    float l[C];
+    auto start_scores = [&](uint32_t to_s) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) l[c] = 0.f;
+        for (int k = 0; k < D / 16; ++k) {
+            const uint32_t in = (k & 3) * 2;  // 32 bytes on within the swizzled rows
+            mma(to_s, dk + (k >> 2) * (kHalfBytes >> 4) + in, dq + (k >> 2) * (N * 128 >> 4) + in, kShape<N>, k > 0);
+        }
+        mma_done(bar_s);
+    };
+    if (tid == 0) start_scores(ts);
+
+    unsigned long long l[C / 2];  // of two columns each, as packed fp32
+#pragma unroll
+    for (int c = 0; c < C / 2; ++c) l[c] = 0;
     bool alive = true;
-    uint32_t phase = 0;  // of both barriers, per tile
+    uint32_t phase = 0;  // of both barriers, per tile; also the tile's S^T
     for (int t0 = first; t0 < last; t0 += kTok, phase ^= 1) {
         const bool more = t0 + kTok < last;
-        put(sk, kw);
-        if (more) fetch_k(t0 + kTok);
-        publish_smem();
-        tmem_fence_before();
-        __syncthreads();
-        if (tid == 0) {
-            tmem_fence_after();
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint32_t in = (k & 3) * 2;  // 32 bytes on within the swizzled rows
-                mma(ts, dk + (k >> 2) * (kHalfBytes >> 4) + in, dq + (k >> 2) * (N * 128 >> 4) + in, kShape<N>, k > 0);
-            }
-            mma_done(bar_s);
+        const uint32_t s_now = ts + phase * N;
+        alive = alive && wait_for(bar_s, phase);  // S is there, K's buffer free
+        tmem_fence_after();
+        if (more) {
+            put(sk, kw);
+            if (t0 + 2 * kTok < last) fetch_k(t0 + 2 * kTok);
         }
         if (t0 > first) alive = alive && wait_for(bar_o, phase ^ 1);  // V's and W's buffers are free
         put(sv, vw);
         if (more) fetch_v(t0 + kTok);
+        if (tid < 8) {  // pages of the tile after the next two (read after this tile's barriers)
+            keep_entry(t0 + 3 * kTok, tid, entry);
+            entry = page_entry(t0 + 4 * kTok, tid);
+        }
 
-        alive = alive && wait_for(bar_s, phase);
-        tmem_fence_after();
         const int tok = t0 + tl;
         const bool past = tok >= last || bad;
-        if (bad && tok < last) raise_flag(a.err, LQ_EF_PAGE);
         const float kx = ks * qk, lv = lg2(vs), rvs = past ? 0.f : rcp(vs);
         if (more) fetch_scales(t0 + kTok);
         uint32_t hidden = past ? 0xffffffffu : 0u;  // columns that do not see the token
@@ -319,29 +348,36 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
                 hidden |= (uint32_t)!paged_sees(a, b, a.by_group.div(row0 + col0 + c), tok - drafts) << c;
         float x[C];
         auto scores = [&]() {
-            tmem_load<C>(ts + my_lanes + col0, x);
+            tmem_load<C>(s_now + my_lanes + col0, x);
+            const unsigned long long mul = f2_pack(kx, kx), add = f2_pack(lv, lv);
 #pragma unroll
-            for (int c = 0; c < C; ++c) x[c] = fmaf(x[c], kx, lv);
+            for (int c = 0; c < C; c += 2) f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), mul, add), x[c], x[c + 1]);
             if (__any_sync(0xffffffffu, hidden != 0)) {
 #pragma unroll
                 for (int c = 0; c < C; ++c) x[c] = hidden >> c & 1 ? -INFINITY : x[c];
             }
         };
         auto less_reference = [&]() {
-            bool grow = false;
+            float top = -INFINITY;
 #pragma unroll
             for (int c = 0; c < C; c += 4) {
-                const float4 m = *reinterpret_cast<const float4 *>(sm.m + col0 + c);
-                x[c] -= m.x;
-                x[c + 1] -= m.y;
-                x[c + 2] -= m.z;
-                x[c + 3] -= m.w;
-                grow |= fmaxf(fmaxf(x[c], x[c + 1]), fmaxf(x[c + 2], x[c + 3])) > kRefSlack;
+                const float4 m = *reinterpret_cast<const float4 *>(sm.minus_m + col0 + c);
+                f2_unpack(f2_add(f2_pack(x[c], x[c + 1]), f2_pack(m.x, m.y)), x[c], x[c + 1]);
+                f2_unpack(f2_add(f2_pack(x[c + 2], x[c + 3]), f2_pack(m.z, m.w)), x[c + 2], x[c + 3]);
+                top = fmaxf(fmaxf(fmaxf(top, x[c]), fmaxf(x[c + 1], x[c + 2])), x[c + 3]);
             }
-            return grow;
+            return top > kRefSlack;
         };
         scores();
-        if (__syncthreads_or(less_reference())) {
+        const bool grow = less_reference();
+        publish_smem();
+        tmem_fence_before();
+        const bool move = __syncthreads_or(grow);
+        if (tid == 0 && more) {
+            tmem_fence_after();
+            start_scores(ts + (phase ^ 1) * N);
+        }
+        if (move) {
             // the tile's column maxima move the references; l and O follow
             scores();
 #pragma unroll
@@ -349,21 +385,19 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
                 float top = x[c];
 #pragma unroll
                 for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                if (lane == 0) sm.red[warp][c] = top;
+                if (lane == 0) sm.red[warp & 3][col0 + c] = top;
             }
             __syncthreads();
             for (int n = tid; n < N; n += kThreads) {
-                const int g = n / C, c = n % C;
-                const float top = fmaxf(fmaxf(sm.red[4 * g][c], sm.red[4 * g + 1][c]),
-                                        fmaxf(sm.red[4 * g + 2][c], sm.red[4 * g + 3][c]));
-                const float next = fmaxf(sm.m[n], top - kRefBelow);
-                sm.f[n] = ex2(sm.m[n] - next);
-                sm.m[n] = next;
+                const float top = fmaxf(fmaxf(sm.red[0][n], sm.red[1][n]), fmaxf(sm.red[2][n], sm.red[3][n]));
+                const float m = -sm.minus_m[n], next = fmaxf(m, top - kRefBelow);
+                sm.f[n] = ex2(m - next);
+                sm.minus_m[n] = -next;
             }
             __syncthreads();
             less_reference();
 #pragma unroll
-            for (int c = 0; c < C; ++c) l[c] *= sm.f[col0 + c];
+            for (int c = 0; c < C; c += 2) l[c / 2] = f2_mul(l[c / 2], f2_pack(sm.f[col0 + c], sm.f[col0 + c + 1]));
             if (t0 > first) {  // this warp's lanes (channels) and columns of O; its MMAs are done
                 float o[C];
                 tmem_load<C>(to + my_lanes + col0, o);
@@ -372,18 +406,20 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
                 tmem_store<C>(to + my_lanes + col0, o);
             }
         }
-        // weights: column c of this token, K-major rows of 64 tokens
-        const uint32_t at = sp + (tl >> 6) * (N * 128) + (tl & 7) * 2;
-        const uint32_t chunk = tl >> 3 & 7;
+        // weights: this token's row of columns
+        const unsigned long long rvs2 = f2_pack(rvs, rvs);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
+        for (int c = 0; c < C; c += 8) {
+            uint32_t pair[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float w0 = ex2(x[c + 2 * i]), w1 = ex2(x[c + 2 * i + 1]);
+                l[c / 2 + i] = f2_fma(f2_pack(w0, w1), rvs2, l[c / 2 + i]);
+                const __half2 h2 = __floats2half2_rn(w0, w1);
+                pair[i] = *reinterpret_cast<const uint32_t *>(&h2);
+            }
             const int n = col0 + c;
-            const float w = ex2(x[c]);
-            l[c] = fmaf(w, rvs, l[c]);
-            const __half hw = __float2half_rn(w);
-            asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + n * 128 + ((chunk ^ (n & 7)) << 4)),
-                         "h"(*reinterpret_cast<const uint16_t *>(&hw))
-                         : "memory");
+            store16(sp + (n >> 6) * kHalfBytes + tl * 128 + (((n >> 3 & 7) ^ (tl & 7)) << 4), pair);
         }
         publish_smem();
         tmem_fence_before();
@@ -392,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
             tmem_fence_after();
 #pragma unroll
             for (int k = 0; k < kTok / 16; ++k)
-                mma(to, dv + k * (2048 >> 4), dp + (k >> 2) * (N * 128 >> 4) + (k & 3) * 2, kShape<N> | kTransposeA,
+                mma(to, dv + k * (2048 >> 4), dp + k * (2048 >> 4), kShape<N> | kTransposeA | kTransposeB,
                     t0 > first || k > 0);
             mma_done(bar_o);
         }
@@ -404,9 +440,12 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
     // denominators over the 128 tokens, then O: a lane is a channel
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+        float l0, l1;
+        f2_unpack(l[c / 2], l0, l1);
+        float sum = c & 1 ? l1 : l0;
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
-        if (lane == 0) sm.red[warp][c] = l[c];
+        for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) sm.red[warp & 3][col0 + c] = sum;
     }
     float o[C];
     tmem_load<C>(to + my_lanes + col0, o);
@@ -418,9 +457,9 @@ __global__ void __launch_bounds__(kThreads, N <= 16 ? 3 : 2)
         for (int c = 0; c < C; ++c) rows[(col0 + c) * D + d] = o[c];
     __syncthreads();
     for (int e = tid; e < live * D; e += kThreads) {
-        const int n = e / D, g = n / C, c = n % C;
-        const float den = (sm.red[4 * g][c] + sm.red[4 * g + 1][c]) + (sm.red[4 * g + 2][c] + sm.red[4 * g + 3][c]);
-        paged_emit<BF16, D>(a, b, h, row0 + n, e % D, blockIdx.x, rows[e], den, sm.m[n]);
+        const int n = e / D;
+        const float den = (sm.red[0][n] + sm.red[1][n]) + (sm.red[2][n] + sm.red[3][n]);
+        paged_emit<BF16, D>(a, b, h, row0 + n, e % D, blockIdx.x, rows[e], den, -sm.minus_m[n]);
     }
     tmem_fence_before();
     __syncthreads();
@@ -435,7 +474,7 @@ int launch_n(const PagedAttnArgs &a, uint32_t batch, cudaStream_t st) {
         cudaSuccess)
         return LQ_ERR_CUDA;
     paged_attn_tc_kernel<BF16, D, N>
-        <<<dim3(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, N), batch), kThreads, smem, st>>>(a);
+        <<<dim3(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, N), batch), kThreads<N>, smem, st>>>(a);
     return check_launch();
 }
 
@@ -443,6 +482,8 @@ template <bool BF16, int D>
 int launch_d(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st) {
     if (tile == 16) return launch_n<BF16, D, 16>(a, batch, st);
     if (tile == 32) return launch_n<BF16, D, 32>(a, batch, st);
+    if constexpr (D == 128)
+        if (tile == 128) return launch_n<BF16, D, 128>(a, batch, st);
     return launch_n<BF16, D, 64>(a, batch, st);
 }
 
