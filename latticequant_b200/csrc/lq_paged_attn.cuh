@@ -30,10 +30,10 @@ struct PagedAttnArgs {
     uint32_t *err;
 };
 
-// The reference M of the base-2 weights 2^(x - M): "none yet", how far an x
-// may exceed it (fp16 holds 2^15), and how far below the maximum it is put
-// (headroom that keeps smaller weights out of fp16's subnormals).
-constexpr float kNoRef = -1e30f, kRefSlack = 14.f, kRefBelow = 6.f;
+// The reference M of the base-2 weights 2^(x - M): "none yet", and how far an x
+// may exceed it (fp16 holds 2^15; a weight under 2^-14 of the reference loses
+// at most 2^-25 of it).  It is put at a maximum, so it rarely moves again.
+constexpr float kNoRef = -1e30f, kRefSlack = 15.f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

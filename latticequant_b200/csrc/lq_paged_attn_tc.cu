@@ -38,6 +38,19 @@ __device__ __forceinline__ void store16(uint32_t addr, const uint32_t (&v)[4]) {
                  : "memory");
 }
 
+// Read-only global loads that stay where they are written (the compiler would
+// sink them to their use, a tile later, to save registers).
+__device__ __forceinline__ uint4 load_early(const uint4 *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float load_early(const float *p) {
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+
 // Matrix descriptor of a 128-byte-swizzled operand: lead and stride in bytes.
 __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride) {
     return (uint64_t)(addr >> 4 & 0x3fffu) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 |
@@ -253,18 +266,18 @@ __global__ void __launch_bounds__(kThreads<N>, N <= 16 ? 3 : N <= 64 ? 2 : 1)
     auto fetch_k = [&](int t0) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r)
-            kw[r] = __ldg(reinterpret_cast<const uint4 *>(kbase + row_of(t0, drow + r * kRowStep) * W));
+            kw[r] = load_early(reinterpret_cast<const uint4 *>(kbase + row_of(t0, drow + r * kRowStep) * W));
     };
     auto fetch_v = [&](int t0) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r)
-            vw[r] = __ldg(reinterpret_cast<const uint4 *>(kbase + (row_of(t0, drow + r * kRowStep) + side) * W));
+            vw[r] = load_early(reinterpret_cast<const uint4 *>(kbase + (row_of(t0, drow + r * kRowStep) + side) * W));
     };
     auto fetch_scales = [&](int t0) {
         const int64_t row = row_of(t0, tl);
         bad = page_of(t0, tl) < 0;
-        ks = __ldg(sbase + row);
-        vs = __ldg(sbase + row + side);
+        ks = load_early(sbase + row);
+        vs = load_early(sbase + row + side);
     };
     // Decoded rows into an operand.  At D = 128 the two 64-channel halves fall on the same banks, so the
     // threads of the upper one take their words in the order 2, 3, 0, 1.
@@ -390,7 +403,7 @@ __global__ void __launch_bounds__(kThreads<N>, N <= 16 ? 3 : N <= 64 ? 2 : 1)
             __syncthreads();
             for (int n = tid; n < N; n += kThreads) {
                 const float top = fmaxf(fmaxf(sm.red[0][n], sm.red[1][n]), fmaxf(sm.red[2][n], sm.red[3][n]));
-                const float m = -sm.minus_m[n], next = fmaxf(m, top - kRefBelow);
+                const float m = -sm.minus_m[n], next = fmaxf(m, top);
                 sm.f[n] = ex2(m - next);
                 sm.minus_m[n] = -next;
             }
