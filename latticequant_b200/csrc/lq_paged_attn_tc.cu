@@ -263,21 +263,23 @@ __global__ void __launch_bounds__(kThreads<N>, N <= 16 ? 3 : N <= 64 ? 2 : 1)
     uint4 kw[RPT], vw[RPT];
     float ks, vs;
     bool bad;
-    auto fetch_k = [&](int t0) {
+    // K of the tile at tk, V and scales of the one at tv: all page lookups, then all loads (a lookup
+    // behind a load in flight would wait for it)
+    auto fetch = [&](int tk, int tv) {
+        int64_t rk[RPT], rv[RPT];
 #pragma unroll
-        for (int r = 0; r < RPT; ++r)
-            kw[r] = load_early(reinterpret_cast<const uint4 *>(kbase + row_of(t0, drow + r * kRowStep) * W));
-    };
-    auto fetch_v = [&](int t0) {
+        for (int r = 0; r < RPT; ++r) {
+            rk[r] = tk < last ? row_of(tk, drow + r * kRowStep) : 0;
+            rv[r] = tv < last ? row_of(tv, drow + r * kRowStep) : 0;
+        }
+        const int64_t rs = tv < last ? row_of(tv, tl) : 0;
+        bad = tv < last && page_of(tv, tl) < 0;
 #pragma unroll
-        for (int r = 0; r < RPT; ++r)
-            vw[r] = load_early(reinterpret_cast<const uint4 *>(kbase + (row_of(t0, drow + r * kRowStep) + side) * W));
-    };
-    auto fetch_scales = [&](int t0) {
-        const int64_t row = row_of(t0, tl);
-        bad = page_of(t0, tl) < 0;
-        ks = load_early(sbase + row);
-        vs = load_early(sbase + row + side);
+        for (int r = 0; r < RPT; ++r) kw[r] = load_early(reinterpret_cast<const uint4 *>(kbase + rk[r] * W));
+#pragma unroll
+        for (int r = 0; r < RPT; ++r) vw[r] = load_early(reinterpret_cast<const uint4 *>(kbase + (rv[r] + side) * W));
+        ks = load_early(sbase + rs);
+        vs = load_early(sbase + rs + side);
     };
     // Decoded rows into an operand.  At D = 128 the two 64-channel halves fall on the same banks, so the
     // threads of the upper one take their words in the order 2, 3, 0, 1.
@@ -305,11 +307,9 @@ __global__ void __launch_bounds__(kThreads<N>, N <= 16 ? 3 : N <= 64 ? 2 : 1)
     if (tid < 24) keep_entry(first + tid / 8 * kTok, tid % 8, page_entry(first + tid / 8 * kTok, tid % 8));
     int entry = tid < 8 ? page_entry(first + 3 * kTok, tid) : 0;  // on its way to the ring
     __syncthreads();
-    fetch_k(first);
-    fetch_v(first);
-    fetch_scales(first);
+    fetch(first, first);
     put(sk, kw);
-    if (first + kTok < last) fetch_k(first + kTok);
+    fetch(first + kTok, first);
     publish_smem();
     tmem_fence_before();
     __syncthreads();
@@ -338,22 +338,18 @@ __global__ void __launch_bounds__(kThreads<N>, N <= 16 ? 3 : N <= 64 ? 2 : 1)
         const uint32_t s_now = ts + phase * N;
         alive = alive && wait_for(bar_s, phase);  // S is there, K's buffer free
         tmem_fence_after();
-        if (more) {
-            put(sk, kw);
-            if (t0 + 2 * kTok < last) fetch_k(t0 + 2 * kTok);
-        }
+        if (more) put(sk, kw);
         if (t0 > first) alive = alive && wait_for(bar_o, phase ^ 1);  // V's and W's buffers are free
         put(sv, vw);
-        if (more) fetch_v(t0 + kTok);
+        const int tok = t0 + tl;
+        const bool past = tok >= last || bad;
+        const float kx = ks * qk, lv = lg2(vs), rvs = past ? 0.f : rcp(vs);
+        fetch(t0 + 2 * kTok, t0 + kTok);
         if (tid < 8) {  // pages of the tile after the next two (read after this tile's barriers)
             keep_entry(t0 + 3 * kTok, tid, entry);
             entry = page_entry(t0 + 4 * kTok, tid);
         }
 
-        const int tok = t0 + tl;
-        const bool past = tok >= last || bad;
-        const float kx = ks * qk, lv = lg2(vs), rvs = past ? 0.f : rcp(vs);
-        if (more) fetch_scales(t0 + kTok);
         uint32_t hidden = past ? 0xffffffffu : 0u;  // columns that do not see the token
         if (tok >= drafts && !past)
 #pragma unroll 1
