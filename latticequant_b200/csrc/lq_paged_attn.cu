@@ -406,12 +406,12 @@ struct Plan {
     uint32_t splits;
 };
 
-Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len, int head_dim) {
+Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
     Plan p;
-    p.tile = rows <= kFewRows ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || head_dim == 64 ? 64 : 128;
+    p.tile = rows <= kFewRows ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     const int64_t least = p.tile == 8 ? 64 : 128;
     const int64_t units = batch * n_heads * ceil_div(rows, p.tile);  // CTAs without a split
-    const int64_t want = ceil_div((int64_t)148 * (p.tile == 8 ? 16 : p.tile == 16 ? 12 : p.tile <= 64 ? 8 : 4), units);
+    const int64_t want = ceil_div((int64_t)148 * (p.tile == 8 ? 16 : 4), units);
     const int64_t tokens = max_len < 1 ? 1 : max_len;
     p.chunk = ceil_div(ceil_div(tokens, want), least) * least;
     p.splits = (uint32_t)ceil_div(tokens, p.chunk);
@@ -432,7 +432,7 @@ static bool paged_shape_ok(int64_t batch, int n_heads, int group, int64_t n_quer
 extern "C" size_t lq_paged_attention_workspace(int64_t batch, int n_heads, int group, int64_t n_query, int head_dim,
                                                int64_t max_len) {
     if (!paged_shape_ok(batch, n_heads, group, n_query, head_dim) || max_len < 0) return 0;
-    const Plan p = plan(batch, n_heads, n_query * group, max_len, head_dim);
+    const Plan p = plan(batch, n_heads, n_query * group, max_len);
     return p.splits > 1 ? (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 2) * 4 : 0;
 }
 
@@ -449,12 +449,13 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
         return LQ_ERR_INVALID;
     if (batch == 0) return LQ_OK;
     if (!q || !codes || !scales || (!table && table_width > 0) || !lens || !out) return LQ_ERR_INVALID;
-    const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(codes);
+    const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(codes) |
+                         reinterpret_cast<uintptr_t>(scales);
     if ((al & 15) != 0 || ((q_stride_b | q_stride_h | q_stride_t) & 7) != 0) return LQ_ERR_INVALID;
     // tokens past max_len would have no split: the caller's bound is the table's at most
     const int64_t cap = table_width * page_tokens;
     const int64_t bound = max_len < cap ? max_len : cap;
-    const Plan p = plan(batch, n_heads, n_query * group, bound, head_dim);
+    const Plan p = plan(batch, n_heads, n_query * group, bound);
     if (p.splits > 1) {
         if (!workspace) return LQ_ERR_INVALID;
         if (workspace_bytes < (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 2) * 4)
