@@ -126,7 +126,7 @@ template <bool BF16, int D, int NT>
 __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int KW = D / 32, VW = D / 64, W = D / 8, MT = D / 16;
     constexpr int ROWS = 8 * NT;
-    extern __shared__ __align__(16) float sm[];  // [warps][ROWS][D + 2]
+    extern __shared__ __align__(16) float sm[];  // [warps][ROWS][D + 4]
     const int warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t b = blockIdx.z, rt = blockIdx.y / a.n_heads, h = blockIdx.y - rt * a.n_heads;
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
     }
 
     // the warps' statistics and outputs, merged in warp order
-    constexpr int rs = D + 2;
+    constexpr int rs = D + 4;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -346,56 +346,71 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
             }
         }
     __syncthreads();
-    const uint32_t live = min((uint32_t)ROWS, a.rows - row0);
-    for (uint32_t e = threadIdx.x; e < live * D; e += 32 * kWarps) {
-        const uint32_t r = e / D, d = e % D;
-        float mx = kNoRef;
+    for (uint32_t r = warp; r < min((uint32_t)ROWS, a.rows - row0); r += kWarps) {
+        float mx = kNoRef, ld = 0.f, od[D / 32] = {};
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm[(w * ROWS + r) * rs + D]);
-        float od = 0.f, ld = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float *src = sm + (w * ROWS + r) * rs;
             const float f = ex2(src[D] - mx);
-            od = fmaf(src[d], f, od);
             ld = fmaf(src[D + 1], f, ld);
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) od[k] = fmaf(src[lane * (D / 32) + k], f, od[k]);
         }
-        paged_emit<BF16, D>(a, b, h, row0 + r, d, blockIdx.x, od, ld, mx);
+        paged_emit_row<BF16, D>(a, b, h, row0 + r, blockIdx.x, od, ld, mx);
     }
 }
 
-// One row per group of D threads: the splits' partial results joined in split order.
+// A warp per row: the splits' partial results joined in split order.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a, uint32_t n_rows) {
-    const uint32_t i = blockIdx.x * (128 / D) + threadIdx.x / D, d = threadIdx.x % D;
+    const uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (i >= n_rows) return;
+    after_previous();
     const uint32_t bh = i / a.rows, r = i - bh * a.rows;
     const uint32_t b = bh / a.n_heads, h = bh - b * a.n_heads;
-    const float *p = a.part + ((int64_t)bh * a.splits * a.rows + r) * (D + 2);
-    const int64_t step = (int64_t)a.rows * (D + 2);
-    const int64_t len = paged_len(a, b);
-    const uint32_t used = (uint32_t)ceil_div(len, a.chunk);
-    float mx = kNoRef;
-    for (uint32_t s = 0; s < used; ++s) mx = fmaxf(mx, p[s * step + D]);
-    float od = 0.f, ld = 0.f;
+    const float *p = paged_part<D>(a, bh, 0);
+    const int64_t step = (int64_t)a.rows * (D + 4);
+    const uint32_t used = (uint32_t)ceil_div(paged_len(a, b), a.chunk);
+    float m = kNoRef;
+    for (uint32_t s = lane; s < used; s += 32) m = fmaxf(m, p[s * step + (int64_t)a.rows * D + 2 * r]);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f, od[D / 32] = {};
+#pragma unroll 4
     for (uint32_t s = 0; s < used; ++s) {
-        const float f = ex2(p[s * step + D] - mx);
-        od = fmaf(p[s * step + d], f, od);
-        ld = fmaf(p[s * step + D + 1], f, ld);
+        const float *q = p + s * step;
+        const float2 st = *reinterpret_cast<const float2 *>(q + (int64_t)a.rows * D + 2 * r);
+        const float f = ex2(st.x - m);
+        l = fmaf(st.y, f, l);
+        float v[D / 32];
+        if constexpr (D == 128) {
+            const float4 x = *reinterpret_cast<const float4 *>(q + (int64_t)r * D + lane * 4);
+            v[0] = x.x;
+            v[1] = x.y;
+            v[2] = x.z;
+            v[3] = x.w;
+        } else {
+            const float2 x = *reinterpret_cast<const float2 *>(q + (int64_t)r * D + lane * 2);
+            v[0] = x.x;
+            v[1] = x.y;
+        }
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) od[k] = fmaf(v[k], f, od[k]);
     }
-    paged_store<BF16, D>(a, b, h, r, d, od, ld, mx);
+    paged_store_row<BF16, D>(a, b, h, r, od, l, m);
 }
 
 template <bool BF16, int D>
 int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st) {
     if (tile == 8)
         paged_attn_kernel<BF16, D, 1><<<dim3(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, 8), batch), 32 * kWarps,
-                                        kWarps * 8 * (D + 2) * 4, st>>>(a);
+                                        kWarps * 8 * (D + 4) * 4, st>>>(a);
     const int status = tile == 8 ? check_launch() : launch_paged_tc(a, BF16, D, tile, batch, st);
     if (status != LQ_OK || a.splits == 1) return status;
     const uint32_t n = batch * a.n_heads * a.rows;
-    paged_combine_kernel<BF16, D><<<(unsigned)ceil_div(n, 128 / D), 128, 0, st>>>(a, n);
-    return check_launch();
+    return launch_overlapped(paged_combine_kernel<BF16, D>, dim3((unsigned)ceil_div(n, 4)), 128, 0, st, a, n);
 }
 
 // Rows of a CTA and tokens of a split: enough CTAs for about four rounds of
@@ -433,7 +448,7 @@ extern "C" size_t lq_paged_attention_workspace(int64_t batch, int n_heads, int g
                                                int64_t max_len) {
     if (!paged_shape_ok(batch, n_heads, group, n_query, head_dim) || max_len < 0) return 0;
     const Plan p = plan(batch, n_heads, n_query * group, max_len);
-    return p.splits > 1 ? (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 2) * 4 : 0;
+    return p.splits > 1 ? (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 4) * 4 : 0;
 }
 
 extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
@@ -457,8 +472,8 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
     const int64_t bound = max_len < cap ? max_len : cap;
     const Plan p = plan(batch, n_heads, n_query * group, bound);
     if (p.splits > 1) {
-        if (!workspace) return LQ_ERR_INVALID;
-        if (workspace_bytes < (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 2) * 4)
+        if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return LQ_ERR_INVALID;
+        if (workspace_bytes < (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 4) * 4)
             return LQ_ERR_CAPACITY;
     }
     PagedAttnArgs a{};

@@ -26,7 +26,7 @@ struct PagedAttnArgs {
     float qk_log2;  // sm_scale * log2(e)
     void *out;      // [batch][n_heads * group][T][D] in q's type
     float *lse;     // [batch][n_heads * group][T] natural log, may be NULL
-    float *part;    // [batch][n_heads][splits][rows][D + 2]: o, reference, denominator
+    float *part;    // [batch][n_heads][splits] of paged_part
     uint32_t *err;
 };
 
@@ -61,31 +61,51 @@ __device__ __forceinline__ bool paged_sees(const PagedAttnArgs &a, uint32_t b, u
     return a.mask ? a.mask[b * a.mask_stride_b + (int64_t)t * a.T + j] != 0 : j <= (int64_t)t;
 }
 
-// Channel d of row r from its weighted sum, denominator and reference.
-template <bool BF16, int D>
-__device__ __forceinline__ void paged_store(const PagedAttnArgs &a, uint32_t b, uint32_t h, uint32_t r, uint32_t d,
-                                            float o, float l, float m) {
-    const uint32_t t = a.by_group.div(r), qh = h * a.group + (r - t * a.group);
-    const int64_t row = ((int64_t)b * a.n_heads * a.group + qh) * a.T + t;
-    // a row that sees nothing has l = 0 (a NaN denominator stays NaN)
-    Elem<BF16 ? LQ_BF16 : LQ_F16>::store(a.out, row * D + d, l == 0.f ? 0.f : o * kCodeUnit / l);
-    if (a.lse && d == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+// Partial results of one (sequence, head, split): o [rows][D], then [rows] of
+// (reference, denominator), in rows * (D + 4) floats so that rows stay 16-byte aligned.
+template <int D>
+__device__ __forceinline__ float *paged_part(const PagedAttnArgs &a, uint32_t bh, uint32_t split) {
+    return a.part + ((int64_t)bh * a.splits + split) * a.rows * (D + 4);
 }
 
-// paged_store, or the split's partial result.
+// Row r from its weighted sums (a warp: D / 32 channels a lane), denominator and reference.
 template <bool BF16, int D>
-__device__ __forceinline__ void paged_emit(const PagedAttnArgs &a, uint32_t b, uint32_t h, uint32_t r, uint32_t d,
-                                           uint32_t split, float o, float l, float m) {
+__device__ __forceinline__ void paged_store_row(const PagedAttnArgs &a, uint32_t b, uint32_t h, uint32_t r,
+                                                const float (&o)[D / 32], float l, float m) {
+    const uint32_t lane = threadIdx.x & 31, t = a.by_group.div(r), qh = h * a.group + (r - t * a.group);
+    const int64_t row = ((int64_t)b * a.n_heads * a.group + qh) * a.T + t;
+    // a row that sees nothing has l = 0 (a NaN denominator stays NaN)
+    const float inv = l == 0.f ? 0.f : kCodeUnit / l;
+    uint32_t w[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        if constexpr (BF16) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(o[2 * i] * inv, o[2 * i + 1] * inv);
+            w[i] = *reinterpret_cast<const uint32_t *>(&p);
+        } else {
+            const __half2 p = __floats2half2_rn(o[2 * i] * inv, o[2 * i + 1] * inv);
+            w[i] = *reinterpret_cast<const uint32_t *>(&p);
+        }
+    }
+    uint32_t *out = static_cast<uint32_t *>(a.out) + (row * D + lane * (D / 32)) / 2;
+    if constexpr (D == 128) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
+    else *out = w[0];
+    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// paged_store_row, or the split's partial result.
+template <bool BF16, int D>
+__device__ __forceinline__ void paged_emit_row(const PagedAttnArgs &a, uint32_t b, uint32_t h, uint32_t r, uint32_t split,
+                                               const float (&o)[D / 32], float l, float m) {
     if (a.splits == 1) {
-        paged_store<BF16, D>(a, b, h, r, d, o, l, m);
+        paged_store_row<BF16, D>(a, b, h, r, o, l, m);
         return;
     }
-    float *p = a.part + (((int64_t)(b * a.n_heads + h) * a.splits + split) * a.rows + r) * (D + 2);
-    p[d] = o;
-    if (d == 0) {
-        p[D] = m;
-        p[D + 1] = l;
-    }
+    const uint32_t lane = threadIdx.x & 31;
+    float *p = paged_part<D>(a, b * a.n_heads + h, split), *po = p + (int64_t)r * D + lane * (D / 32);
+    if constexpr (D == 128) *reinterpret_cast<float4 *>(po) = make_float4(o[0], o[1], o[2], o[3]);
+    else *reinterpret_cast<float2 *>(po) = make_float2(o[0], o[1]);
+    if (lane == 0) *reinterpret_cast<float2 *>(p + (int64_t)a.rows * D + 2 * r) = make_float2(m, l);
 }
 
 // A bf16 pair times the power of two f, as an fp16 pair.

@@ -16,11 +16,12 @@
 //       MMAs read (a decoded block of 8 channels is one 16-byte chunk; V^T is
 //       read from the same token-major layout as an MN-major operand)
 //   two issuers start the two MMAs of every tile
-//   softmax    scores out of TMEM, weights to shared memory, a row of N per
-//       token.  What a tile waits for here is latency, so with up to 32 rows two
-//       sets of 4 warps take the tiles in turn, each with references,
-//       denominators and an O of its own, joined at the end; with 64 rows two
-//       column halves share every tile
+//   softmax    scores out of TMEM, weights to shared memory, a row of N per token
+// What a tile waits for in the last part, and with few rows in decoding, is
+// latency: 16 columns a thread keep enough warps there, with up to 32 rows two
+// sets of softmax warps take the tiles in turn, each with references,
+// denominators and an O of its own that are joined at the end, and with up to
+// 16 two sets of decoders do.
 // so copying, decoding, the tensor cores and the exponentials overlap.
 //
 // M is a reference per row, moved only when an x exceeds it by kRefSlack,
@@ -149,6 +150,10 @@ __device__ __forceinline__ void arrive_warp(uint32_t bar) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) arrive(bar);
 }
+template <class X>
+__device__ __forceinline__ void sync_softmax() {
+    asm volatile("bar.sync 8, %0;" ::"n"(32 * X::kSoftmax) : "memory");
+}
 // Barrier of 128 threads, and its vote.
 __device__ __forceinline__ void sync128(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ bool any128(int id, bool x) {
@@ -165,20 +170,14 @@ __device__ __forceinline__ bool any128(int id, bool x) {
 template <int D, int COLS>
 struct Shape {
     static constexpr int kN = COLS < 16 ? 16 : COLS;   // columns of the MMAs
-    static constexpr int kC = COLS < 32 ? COLS : 32;   // columns of a softmax thread
+    static constexpr int kC = COLS < 16 ? COLS : 16;   // columns of a softmax thread
     static constexpr int kGroups = COLS / kC;          // column groups of 4 warps
     static constexpr int kSets = COLS <= 32 ? 2 : 1;   // of softmax warps, which take the tiles in turn
     static constexpr int kSoftmax = 4 * kGroups * kSets;
-    static constexpr int kDecode = D == 128 && COLS < 32 ? 16 : 8;
-    static constexpr int kThreads = 32 * (kSoftmax + kDecode + 4);  // whole warpgroups: the last has two issuers
-                                                                    // and the producer
-    // Registers of a thread: at launch, and of the three parts afterwards where the launch's share is too
-    // small for softmax (0: as launched).  The parts' sum stays below the launch's.
-    static constexpr int kLaunch = 65536 / kThreads / 8 * 8;
-    static constexpr int kSoftmaxRegs = kC == 32 ? 128 : 0;
-    static constexpr int kDecodeRegs = 80, kIssuerRegs = 56;
-    static_assert(kSoftmaxRegs == 0 || (kSoftmaxRegs >= kLaunch && kDecodeRegs <= kLaunch &&
-                  kSoftmax * kSoftmaxRegs + kDecode * kDecodeRegs + 4 * kIssuerRegs <= kThreads / 32 * kLaunch));
+    static constexpr int kDecodeSets = COLS <= 16 ? 2 : 1;
+    static constexpr int kDecode = 8;                  // warps of a set
+    static constexpr int kIssue = kSoftmax + kDecode * kDecodeSets;  // first of the two issuers and the producer
+    static constexpr int kThreads = 32 * (kIssue + 4);
     static constexpr int kPerRow = D / 32;                  // decoder threads of a token's row, four words each
     static constexpr int kRowStep = 32 * kDecode / kPerRow; // token rows the decoders take at once
     static constexpr int kRows = kTok / kRowStep;           // of a thread
@@ -195,9 +194,10 @@ struct Shape {
 template <class X>
 struct Small {
     uint64_t stage_full[X::kStages], stage_free[X::kStages], k_full[2], k_free[2], v_full[2], v_free[2];
-    uint64_t s_full[2], s_free[2], p_full[X::kSets], p_free[X::kSets];
+    uint64_t s_full[2], s_free[2], p_full[X::kSets], p_free[X::kSets], q_full;
     alignas(16) float minus_m[X::kSets][X::kN];
-    float f[X::kSets][X::kN], red[X::kSets][4][X::kN];
+    alignas(16) float f[X::kSets][X::kN];
+    float red[X::kSets][4][X::kN];
     uint32_t bad[X::kStages];  // bit: a page of the stage's tokens lies outside the pool
     uint32_t tmem, exponent;
 };
@@ -212,15 +212,6 @@ struct Waiter {
         alive = alive && wait_for(smem_u32(&bar), phase & 1);
     }
 };
-
-template <int REGS>
-__device__ __forceinline__ void grow_registers() {
-    if constexpr (REGS > 0) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
-}
-template <int REGS>
-__device__ __forceinline__ void shrink_registers() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
-}
 
 template <bool BF16, int D, int COLS>
 __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
@@ -244,8 +235,10 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
     const int live = (int)min((uint32_t)COLS, a.rows - row0);
     if (first >= last) {  // nothing to read; without a split the rows are still written
         if (a.splits == 1)
-            for (int e = tid; e < live * D; e += kThreads)
-                paged_store<BF16, D>(a, b, h, row0 + e / D, e % D, 0.f, 0.f, kNoRef);
+            for (int n = warp; n < live; n += kThreads / 32) {
+                const float zero[D / 32] = {};
+                paged_emit_row<BF16, D>(a, b, h, row0 + n, 0, zero, 0.f, kNoRef);
+            }
         return;
     }
     const int n_tiles = (last - first + kTok - 1) / kTok;
@@ -260,6 +253,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
         auto init = [](uint64_t &bar, uint32_t n) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&bar)), "r"(n) : "memory");
         };
+        init(sm.q_full, X::kSoftmax);
         for (int i = 0; i < X::kStages; ++i) {
             init(sm.stage_full[i], 1);
             init(sm.stage_free[i], X::kDecode + 4 * X::kGroups);
@@ -281,56 +275,6 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
     }
     for (int n = tid; n < X::kSets * N; n += kThreads) sm.minus_m[n / N][n % N] = -kNoRef;
 
-    // ---- Q: fp16 rows in the decoded blocks' channel order; rows past the last are zero
-    constexpr int kChunks = N * W;  // 16-byte chunks
-    constexpr int kQ = (kChunks + kThreads - 1) / kThreads;
-    float qk = a.qk_log2 * kCodeUnit;
-    {
-        uint4 q[kQ];
-#pragma unroll
-        for (int i = 0; i < kQ; ++i) {
-            const int e = tid + i * kThreads, n = e / W, c = e % W;
-            q[i] = make_uint4(0, 0, 0, 0);
-            if (e < kChunks && n < live) {
-                const uint32_t r = row0 + n, qt = a.by_group.div(r), qh = h * a.group + (r - qt * a.group);
-                q[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
-                                                             qh * a.q_stride_h + qt * a.q_stride_t) + c);
-            }
-        }
-        if constexpr (BF16) {  // a power of two for all rows puts the largest finite value in [2^10, 2^11)
-            uint32_t e = 27;   // (at least 2^-100)
-#pragma unroll
-            for (int i = 0; i < kQ; ++i) {
-                const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t lo = w[k] >> 7 & 0xffu, hi = w[k] >> 23 & 0xffu;
-                    e = max(e, max(lo == 0xffu ? 0u : lo, hi == 0xffu ? 0u : hi));
-                }
-            }
-            e = __reduce_max_sync(0xffffffffu, e);
-            __syncthreads();
-            if (lane == 0) atomicMax(&sm.exponent, e);
-            __syncthreads();
-            e = sm.exponent;
-            const float f = __uint_as_float((264u - e) << 23);
-            qk *= __uint_as_float((e - 10u) << 23);
-#pragma unroll
-            for (int i = 0; i < kQ; ++i)
-                q[i] = make_uint4(bf16_to_f16(q[i].x, f), bf16_to_f16(q[i].y, f), bf16_to_f16(q[i].z, f),
-                                  bf16_to_f16(q[i].w, f));
-        }
-#pragma unroll
-        for (int i = 0; i < kQ; ++i) {
-            const int e = tid + i * kThreads, n = e / W, c = e % W;
-            if (e >= kChunks) break;
-            // pairs (7, 3), (6, 2), (5, 1), (4, 0)
-            const uint32_t v[4] = {__byte_perm(q[i].w, q[i].y, 0x7632), __byte_perm(q[i].w, q[i].y, 0x5410),
-                                   __byte_perm(q[i].z, q[i].x, 0x7632), __byte_perm(q[i].z, q[i].x, 0x5410)};
-            store16(sq + (c >> 3) * (N * 128) + n * 128 + (((c & 7) ^ (n & 7)) << 4), v);
-        }
-    }
-    publish_smem();
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -339,7 +283,56 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
 
     if (warp < X::kSoftmax) {
         // ---- softmax: token tl (a TMEM lane), columns col0.., every kSets-th tile
-        grow_registers<X::kSoftmaxRegs>();
+        // Q: fp16 rows in the decoded blocks' channel order; rows past the last are zero
+        constexpr int kLoaders = 32 * X::kSoftmax, kChunks = N * W;  // 16-byte chunks
+        constexpr int kQ = (kChunks + kLoaders - 1) / kLoaders;
+        float qk = a.qk_log2 * kCodeUnit;
+        {
+            uint4 q[kQ];
+    #pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                const int e = tid + i * kLoaders, n = e / W, c = e % W;
+                q[i] = make_uint4(0, 0, 0, 0);
+                if (e < kChunks && n < live) {
+                    const uint32_t r = row0 + n, qt = a.by_group.div(r), qh = h * a.group + (r - qt * a.group);
+                    q[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
+                                                                 qh * a.q_stride_h + qt * a.q_stride_t) + c);
+                }
+            }
+            if constexpr (BF16) {  // a power of two for all rows puts the largest finite value in [2^10, 2^11)
+                uint32_t e = 27;   // (at least 2^-100)
+    #pragma unroll
+                for (int i = 0; i < kQ; ++i) {
+                    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+    #pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t lo = w[k] >> 7 & 0xffu, hi = w[k] >> 23 & 0xffu;
+                        e = max(e, max(lo == 0xffu ? 0u : lo, hi == 0xffu ? 0u : hi));
+                    }
+                }
+                e = __reduce_max_sync(0xffffffffu, e);
+                if (lane == 0) atomicMax(&sm.exponent, e);
+                sync_softmax<X>();
+                e = sm.exponent;
+                const float f = __uint_as_float((264u - e) << 23);
+                qk *= __uint_as_float((e - 10u) << 23);
+    #pragma unroll
+                for (int i = 0; i < kQ; ++i)
+                    q[i] = make_uint4(bf16_to_f16(q[i].x, f), bf16_to_f16(q[i].y, f), bf16_to_f16(q[i].z, f),
+                                      bf16_to_f16(q[i].w, f));
+            }
+    #pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                const int e = tid + i * kLoaders, n = e / W, c = e % W;
+                if (e >= kChunks) break;
+                // pairs (7, 3), (6, 2), (5, 1), (4, 0)
+                const uint32_t v[4] = {__byte_perm(q[i].w, q[i].y, 0x7632), __byte_perm(q[i].w, q[i].y, 0x5410),
+                                       __byte_perm(q[i].z, q[i].x, 0x7632), __byte_perm(q[i].z, q[i].x, 0x5410)};
+                store16(sq + (c >> 3) * (N * 128) + n * 128 + (((c & 7) ^ (n & 7)) << 4), v);
+            }
+        }
+        publish_smem();
+        arrive_warp(smem_u32(&sm.q_full));
         const int tl = (warp & 3) * 32 + lane, group = (warp >> 2) % X::kGroups, set = (warp >> 2) / X::kGroups;
         const int col0 = group * C, vote = 1 + (warp >> 2);
         const uint32_t my_lanes = (uint32_t)((warp & 3) * 32) << 16, o_at = to + set * N + my_lanes + col0;
@@ -461,30 +454,35 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
         tmem_load<C>(o_at, o);
         tmem_fence_before();
         // all sets are through (every operand has been read), then through shared memory to rows of channels
-        asm volatile("bar.sync 8, %0;" ::"n"(32 * X::kSoftmax) : "memory");
+        sync_softmax<X>();
         float *rows = reinterpret_cast<float *>(buf);
         const int d = (tl & ~7) + (int)(kChannel >> (4 * (tl & 7)) & 15u);
         if (D == 128 || tl < 64)
 #pragma unroll
             for (int c = 0; c < C; ++c) rows[(set * COLS + col0 + c) * D + d] = done > 0 ? o[c] : 0.f;
-        asm volatile("bar.sync 8, %0;" ::"n"(32 * X::kSoftmax) : "memory");
-        for (int e = tid; e < live * D; e += 32 * X::kSoftmax) {
-            const int n = e / D;
-            float m = kNoRef, od = 0.f, den = 0.f;
+        sync_softmax<X>();
+        for (int n = warp; n < live; n += X::kSoftmax) {
+            float m = kNoRef, den = 0.f, w[X::kSets], od[D / 32];
 #pragma unroll
             for (int i = 0; i < X::kSets; ++i) m = fmaxf(m, -sm.minus_m[i][n]);
 #pragma unroll
             for (int i = 0; i < X::kSets; ++i) {
-                const float w = ex2(-sm.minus_m[i][n] - m);
-                den = fmaf((sm.red[i][0][n] + sm.red[i][1][n]) + (sm.red[i][2][n] + sm.red[i][3][n]), w, den);
-                od = fmaf(rows[i * COLS * D + e], w, od);
+                w[i] = ex2(-sm.minus_m[i][n] - m);
+                den = fmaf((sm.red[i][0][n] + sm.red[i][1][n]) + (sm.red[i][2][n] + sm.red[i][3][n]), w[i], den);
             }
-            paged_emit<BF16, D>(a, b, h, row0 + n, e % D, blockIdx.x, od, den, m);
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+                od[k] = 0.f;
+#pragma unroll
+                for (int i = 0; i < X::kSets; ++i)
+                    od[k] = fmaf(rows[(i * COLS + n) * D + lane * (D / 32) + k], w[i], od[k]);
+            }
+            paged_emit_row<BF16, D>(a, b, h, row0 + n, blockIdx.x, od, den, m);
         }
-    } else if (warp < X::kSoftmax + X::kDecode) {
-        // ---- decoders: kRows rows of four words each of K and V
-        if constexpr (X::kSoftmaxRegs > 0) shrink_registers<X::kDecodeRegs>();
-        const int dt = tid - 32 * X::kSoftmax, part = dt % X::kPerRow, drow = dt / X::kPerRow;
+    } else if (warp < X::kIssue) {
+        // ---- decoders: kRows rows of four words each of K and V, every kDecodeSets-th tile
+        const int set = (warp - X::kSoftmax) / X::kDecode, dt = tid - 32 * (X::kSoftmax + set * X::kDecode);
+        const int part = dt % X::kPerRow, drow = dt / X::kPerRow;
         // At D = 128 the two 64-channel halves of an operand fall on the same banks, so the threads of the
         // upper one take their words in the order 2, 3, 0, 1.
         const bool upper = D == 128 && part >= 2;
@@ -509,33 +507,32 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
                 }
             }
         };
-        int stage = 0;
-        uint32_t turn = 0;  // of the stages
-        for (int j = 0; j < n_tiles; ++j) {
-            const int s = j & 1;
+        for (int j = set; j < n_tiles; j += X::kDecodeSets) {
+            const int s = j & 1, stage = j % X::kStages;
             const uint32_t from = stages + stage * X::kStageBytes + dt * 16;
-            wait(sm.stage_full[stage], turn);
-            if (j >= 2) wait(sm.k_free[s], (j >> 1) - 1);
+            if (j >= 2) {
+                wait(sm.k_free[s], (j >> 1) - 1);
+                wait(sm.v_free[s], (j >> 1) - 1);
+            }
+            wait(sm.stage_full[stage], j / X::kStages);
             put(sk + s * X::kTileBytes, from);
             publish_smem();
             arrive_warp(smem_u32(&sm.k_full[s]));
-            if (j >= 2) wait(sm.v_free[s], (j >> 1) - 1);
             put(sv + s * X::kTileBytes, from + X::kWordBytes);
             publish_smem();
-            arrive_warp(smem_u32(&sm.v_full[s]));
-            arrive_warp(smem_u32(&sm.stage_free[stage]));
-            if (++stage == X::kStages) {
-                stage = 0;
-                turn ^= 1;
+            __syncwarp();
+            if (lane == 0) {
+                arrive(smem_u32(&sm.v_full[s]));
+                arrive(smem_u32(&sm.stage_free[stage]));
             }
         }
     } else {
         // ---- the issuers (the first warp starts S, the second O) and the producer
-        if constexpr (X::kSoftmaxRegs > 0) shrink_registers<X::kIssuerRegs>();
-        const int issuer = __shfl_sync(0xffffffffu, warp - X::kSoftmax - X::kDecode, 0);  // uniform
+        const int issuer = __shfl_sync(0xffffffffu, warp - X::kIssue, 0);  // uniform
         const uint32_t one = elect_lane();
         if (issuer == 0) {
             const uint64_t dq = operand(sq, 16, 1024), dk = operand(sk, 16, 1024);
+            wait(sm.q_full, 0);
             for (int j = 0; j < n_tiles; ++j) {
                 const int s = j & 1;
                 wait(sm.k_full[s], j >> 1);
