@@ -41,6 +41,23 @@ inline int launch_overlapped(void (*kernel)(Params...), dim3 grid, unsigned bloc
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, Params(args)...) == cudaSuccess ? check_launch() : LQ_ERR_CUDA;
 }
+// Launch a kernel in clusters of `cluster` CTAs along x (1: none).
+template <class... Params, class... Args>
+inline int launch_clustered(void (*kernel)(Params...), dim3 grid, unsigned cluster, unsigned block, size_t smem,
+                            cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at = {};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, Params(args)...) == cudaSuccess ? check_launch() : LQ_ERR_CUDA;
+}
 // Waits until the previous kernel of the stream has finished and its writes are visible.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the next kernel's CTAs be scheduled once every CTA of this one got here or ended.

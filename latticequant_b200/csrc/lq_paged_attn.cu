@@ -61,6 +61,26 @@ __device__ __forceinline__ void load_words(const uint32_t *p, uint32_t w[N]) {
     }
 }
 
+// The CTAs of a cluster: a barrier that also orders their shared memory, and reads of another's.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(const void *p, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+template <int N>
+__device__ __forceinline__ void load_cluster(uint32_t addr, float (&v)[N]) {
+    if constexpr (N == 4)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                     : "r"(addr)
+                     : "memory");
+    else
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
+}
+
 // What a lane (g = lane / 4, t = lane % 4) reads of a 16-token tile: K words
 // t*KW.. of tokens g and g + 8, V words g*VW.. of tokens 2t, 2t+1, 2t+8,
 // 2t+9, and the scales of tokens g and g + 8.
@@ -345,21 +365,39 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
                 dst[D + 1] = l[n][c];
             }
         }
-    __syncthreads();
-    for (uint32_t r = warp; r < min((uint32_t)ROWS, a.rows - row0); r += kWarps) {
+    // rows in turn to the warps of the CTA, or of the cluster, whose CTAs are then the splits
+    const uint32_t ranks = a.clustered ? a.splits : 1, rank = a.clustered ? blockIdx.x : 0;
+    if (a.clustered) cluster_sync();
+    else __syncthreads();
+    for (uint32_t r = rank + ranks * warp; r < min((uint32_t)ROWS, a.rows - row0); r += ranks * kWarps) {
         float mx = kNoRef, ld = 0.f, od[D / 32] = {};
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm[(w * ROWS + r) * rs + D]);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float *src = sm + (w * ROWS + r) * rs;
-            const float f = ex2(src[D] - mx);
-            ld = fmaf(src[D + 1], f, ld);
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) od[k] = fmaf(src[lane * (D / 32) + k], f, od[k]);
+        for (uint32_t p = lane; p < ranks * kWarps; p += 32) {
+            float st[2];
+            load_cluster(in_cta(sm + ((p % kWarps) * ROWS + r) * rs + D, p / kWarps), st);
+            mx = fmaxf(mx, st[0]);
         }
-        paged_emit_row<BF16, D>(a, b, h, row0 + r, blockIdx.x, od, ld, mx);
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        for (uint32_t q = 0; q < ranks; ++q) {
+            const uint32_t base = in_cta(sm + r * rs, q);
+            float st[kWarps][2], v[kWarps][D / 32];
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                load_cluster(base + (w * ROWS * rs + D) * 4, st[w]);
+                load_cluster(base + (w * ROWS * rs + lane * (D / 32)) * 4, v[w]);
+            }
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = ex2(st[w][0] - mx);
+                ld = fmaf(st[w][1], f, ld);
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) od[k] = fmaf(v[w][k], f, od[k]);
+            }
+        }
+        if (a.clustered) paged_store_row<BF16, D>(a, b, h, row0 + r, od, ld, mx);
+        else paged_emit_row<BF16, D>(a, b, h, row0 + r, blockIdx.x, od, ld, mx);
     }
+    if (a.clustered) cluster_sync();  // nobody leaves while its shared memory is read
 }
 
 // A warp per row: the splits' partial results joined in split order.
@@ -404,22 +442,31 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
 
 template <bool BF16, int D>
 int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st) {
-    if (tile == 8)
-        paged_attn_kernel<BF16, D, 1><<<dim3(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, 8), batch), 32 * kWarps,
-                                        kWarps * 8 * (D + 4) * 4, st>>>(a);
-    const int status = tile == 8 ? check_launch() : launch_paged_tc(a, BF16, D, tile, batch, st);
-    if (status != LQ_OK || a.splits == 1) return status;
+    int status;
+    if (tile == 8) {
+        const dim3 grid(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, 8), batch);
+        status = launch_clustered(paged_attn_kernel<BF16, D, 1>, grid, a.clustered ? a.splits : 1, 32 * kWarps,
+                                  kWarps * 8 * (D + 4) * 4, st, a);
+    } else {
+        status = launch_paged_tc(a, BF16, D, tile, batch, st);
+    }
+    if (status != LQ_OK || a.splits == 1 || a.clustered) return status;
     const uint32_t n = batch * a.n_heads * a.rows;
     return launch_overlapped(paged_combine_kernel<BF16, D>, dim3((unsigned)ceil_div(n, 4)), 128, 0, st, a, n);
 }
 
 // Rows of a CTA and tokens of a split: enough CTAs for about four rounds of
-// the GPU, chunks of a tile of tokens at least.
+// the GPU, chunks of a tile of tokens at least.  Up to kClusterMax splits of
+// the few-rows kernel form a cluster and join over its shared memory, which
+// spares the second launch and the workspace; short contexts take fewer
+// splits for it than would fill the GPU.
 struct Plan {
     int tile;
     int64_t chunk;
     uint32_t splits;
+    bool clustered;
 };
+constexpr int64_t kClusterMax = 8, kClusterTokens = 256;  // splits, and the chunk up to which 8 of them are enough
 
 Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
     Plan p;
@@ -430,7 +477,16 @@ Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
     const int64_t tokens = max_len < 1 ? 1 : max_len;
     p.chunk = ceil_div(ceil_div(tokens, want), least) * least;
     p.splits = (uint32_t)ceil_div(tokens, p.chunk);
+    p.clustered = p.tile == 8 && p.splits > 1 && (p.splits <= kClusterMax || tokens <= kClusterMax * kClusterTokens);
+    if (p.clustered) {  // 2, 4 or 8 CTAs (the last may find nothing to do)
+        p.splits = p.splits <= 2 ? 2 : p.splits <= 4 ? 4 : 8;
+        p.chunk = ceil_div(ceil_div(tokens, p.splits), least) * least;
+    }
     return p;
+}
+
+size_t workspace_of(const Plan &p, int64_t bh_rows, int head_dim) {
+    return p.splits > 1 && !p.clustered ? (size_t)bh_rows * p.splits * (head_dim + 4) * 4 : 0;
 }
 
 }  // namespace
@@ -447,8 +503,7 @@ static bool paged_shape_ok(int64_t batch, int n_heads, int group, int64_t n_quer
 extern "C" size_t lq_paged_attention_workspace(int64_t batch, int n_heads, int group, int64_t n_query, int head_dim,
                                                int64_t max_len) {
     if (!paged_shape_ok(batch, n_heads, group, n_query, head_dim) || max_len < 0) return 0;
-    const Plan p = plan(batch, n_heads, n_query * group, max_len);
-    return p.splits > 1 ? (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 4) * 4 : 0;
+    return workspace_of(plan(batch, n_heads, n_query * group, max_len), batch * n_heads * n_query * group, head_dim);
 }
 
 extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
@@ -471,10 +526,9 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
     const int64_t cap = table_width * page_tokens;
     const int64_t bound = max_len < cap ? max_len : cap;
     const Plan p = plan(batch, n_heads, n_query * group, bound);
-    if (p.splits > 1) {
+    if (const size_t need = workspace_of(p, batch * n_heads * n_query * group, head_dim)) {
         if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return LQ_ERR_INVALID;
-        if (workspace_bytes < (size_t)batch * n_heads * p.splits * n_query * group * (head_dim + 4) * 4)
-            return LQ_ERR_CAPACITY;
+        if (workspace_bytes < need) return LQ_ERR_CAPACITY;
     }
     PagedAttnArgs a{};
     a.q = q;
@@ -499,6 +553,7 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
     a.by_group = FastDiv((uint32_t)group);
     a.chunk = p.chunk;
     a.splits = p.splits;
+    a.clustered = p.clustered;
     a.qk_log2 = sm_scale * kLog2e;
     a.out = out;
     a.lse = lse;

@@ -23,6 +23,7 @@ struct PagedAttnArgs {
     FastDiv by_group;
     int64_t chunk;  // tokens of a split
     uint32_t splits;
+    bool clustered;  // the splits of a row are a cluster and join in its shared memory
     float qk_log2;  // sm_scale * log2(e)
     void *out;      // [batch][n_heads * group][T][D] in q's type
     float *lse;     // [batch][n_heads * group][T] natural log, may be NULL

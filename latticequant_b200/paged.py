@@ -74,6 +74,8 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with a contiguous last dimension, 16-byte aligned, its other strides multiples of 8 elements."""
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t
     *outer, last = t.stride()
     if last == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in outer):
         return t
@@ -98,7 +100,7 @@ def append(codes: torch.Tensor, scales: torch.Tensor, k: torch.Tensor, v: torch.
     k, v = _rows(k), _rows(v)
     ko = vo = None
     if dequantised:
-        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        ko = torch.empty_like(k) if k.is_contiguous() else torch.empty_like(k, memory_format=torch.contiguous_format)
         vo = torch.empty_like(ko)
     call("lq_paged_append", index, k.data_ptr(), v.data_ptr(), dt, n, H, D, *k.stride()[:2], *v.stride()[:2], slots_p,
          n_pages, P, codes.data_ptr(), scales.data_ptr(), _ptr(ko), _ptr(vo), _ptr(err))
@@ -138,7 +140,7 @@ def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, t
         mask_stride = T * T if per_row else 0
     q = _rows(q)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _need(out, dtype, (B, Hq, T, D), "out", index)
     lse = lens.new_empty((B, Hq, T), dtype=_F32) if return_lse else None
@@ -174,8 +176,9 @@ def fork_pages(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, l
     (rows, width), n = table.shape, parents.shape[0]
     table_p, lens_p = _need(table, _I32, (rows, width), "table", index), _need(lens, _I32, (rows,), "lens", index)
     refs_p, parents_p = _need(refs, _I32, (n_pages,), "refs", index), _need(parents, torch.int64, (n,), "parents", index)
-    new_table = table.new_empty((n, width))
-    new_lens = lens.new_empty(n)
+    # (empty_like is the cheaper call)
+    new_table = torch.empty_like(table) if n == rows else table.new_empty((n, width))
+    new_lens = torch.empty_like(lens) if n == rows else lens.new_empty(n)
     new_refs = torch.empty_like(refs)
     need = 4 * (rows + n + n_pages)  # lq_pages_fork_workspace
     ws = refs.new_empty(need // 4)
