@@ -16,12 +16,15 @@
 //       keeps a maximum and a sum of exponentials of its own.  The n best
 //       are kept by a bound: among the largest per-thread maxima of each warp
 //       of the first tile the n-th largest is at most the n-th best of the
-//       row, few logits reach it, and those are collected in shared memory
-//       and ranked by counting.  A collection of more than 2 n is cut to its
-//       n best, the last of which is the new bound.
+//       row.  A 16-byte load whose largest logit reaches the bound (few do) is
+//       put aside whole, in its warp's list; a warp whose list grows long
+//       raises the bound to the n-th largest of the list's maxima and drops
+//       what no longer reaches it.  The warps never wait for one another; in
+//       the end the bound is found again among the lists, and the logits that
+//       reach it are ranked by counting.
 //   beam_merge_kernel  a CTA per sequence joins the parts' statistics and
 //       picks the n best totals the same way.
-// A part with so many equal logits that the collection overflows is ranked by
+// A part with so many equal logits that a list or the ranking overflows is ranked by
 // n rounds of a block-wide maximum instead, over the logits in memory.
 #include "lq_attn_common.cuh"
 
@@ -30,6 +33,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kVecs = 4;  // 16-byte loads of a thread and tile
+constexpr int kAside = 320, kAsideLong = kAside - 32 * kVecs;  // loads a warp's list holds; it is cut when this long
 constexpr int kMaxPicked = 1024, kMaxN = 128, kMaxBeams = 256, kMaxVocab = 1 << 24;
 
 // Order-preserving image of a float: larger x, larger value; 0 for no
@@ -84,13 +88,12 @@ __device__ __forceinline__ void find_bound(uint32_t best, int n, Picker &s) {
     __syncthreads();
 }
 
-__device__ __forceinline__ int pick(Picker &s, uint32_t hi, uint64_t lo) {
+__device__ __forceinline__ void pick(Picker &s, uint32_t hi, uint64_t lo) {
     const int at = atomicAdd(&s.count, 1);
     if (at < kMaxPicked) {
         s.hi[at] = hi;
         s.lo[at] = lo;
     }
-    return at;
 }
 
 // emit(rank, key) for the n largest picked keys (all distinct); false: too many were picked.
@@ -140,29 +143,13 @@ __device__ void rank_by_rounds(Picker &s, int n, Best best_below, Emit emit) {
     }
 }
 
-// Keep the n best of the s.count <= kMaxPicked picked keys, and make the last of them the bound.
-__device__ __forceinline__ void cut_picked(Picker &s, int n) {
-    const int c = s.count;
-    uint64_t mine[kMaxPicked / kThreads];
-    int at[kMaxPicked / kThreads];
-#pragma unroll
-    for (int q = 0; q < kMaxPicked / kThreads; ++q) {
-        const int i = threadIdx.x + q * kThreads;
-        mine[q] = i < c ? s.lo[i] : 0;
-        at[q] = i < c ? 0 : kMaxPicked;
-        if (i < c)
-            for (int j = 0; j < c; ++j) at[q] += s.lo[j] > mine[q];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kMaxPicked / kThreads; ++q)
-        if (at[q] < n) {
-            s.lo[at[q]] = mine[q];
-            if (at[q] == n - 1) s.bound = (uint32_t)(mine[q] >> 24);
-        }
-    if (threadIdx.x == 0) s.count = min(c, n);
-    __syncthreads();
-}
+// The loads that the warps put aside.
+struct Aside {
+    uint4 data[kWarps][kAside];
+    int word[kWarps][kAside];  // of element 0
+    int count[kWarps];
+    int overflow;
+};
 
 struct BeamArgs {
     const void *logits;
@@ -215,13 +202,64 @@ __device__ __forceinline__ float exp_of(float x) {
     return y;
 }
 
+// A warp's list cut by the n-th largest of its loads' maxima, which becomes the bound for all.
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_constant__ BeamArgs a) {
+__device__ __noinline__ void cut_aside(Aside &x, int warp, int n, uint32_t *bound) {
+    const int lane = threadIdx.x & 31, c = x.count[warp];
+    uint32_t top[kAside / 32];
+#pragma unroll
+    for (int q = 0; q < kAside / 32; ++q) {
+        const int i = lane + 32 * q;
+        top[q] = i < c ? ordered(largest<DT>(x.data[warp][i])) : 0u;
+    }
+    uint32_t nth = 0;
+    for (int r = 0; r < n; ++r) {  // n rounds of a maximum, one load leaving in each
+        uint32_t mine = 0;
+#pragma unroll
+        for (int q = 0; q < kAside / 32; ++q) mine = max(mine, top[q]);
+        nth = __reduce_max_sync(0xffffffffu, mine);
+        const bool first = lane == __ffs(__ballot_sync(0xffffffffu, mine == nth)) - 1;
+        bool gone = !first;
+#pragma unroll
+        for (int q = 0; q < kAside / 32; ++q)
+            if (!gone && top[q] == nth) {
+                top[q] = 0;
+                gone = true;
+            }
+    }
+    int kept = 0;
+    for (int i0 = 0; i0 < c; i0 += 32) {
+        const int i = i0 + lane;
+        const uint4 d = x.data[warp][min(i, kAside - 1)];
+        const int w = x.word[warp][min(i, kAside - 1)];
+        const bool keep = i < c && ordered(largest<DT>(d)) >= max(nth, 1u);
+        const uint32_t all = __ballot_sync(0xffffffffu, keep);
+        if (keep) {  // at or before its old place
+            const int at = kept + __popc(all & ((1u << lane) - 1));
+            x.data[warp][at] = d;
+            x.word[warp][at] = w;
+        }
+        kept += __popc(all);
+        __syncwarp();
+    }
+    if (lane == 0) {
+        x.count[warp] = kept;
+        atomicMax(bound, nth);
+        if (kept > kAsideLong) x.overflow = 1;  // as many equal maxima
+    }
+    __syncwarp();
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 3) beam_part_kernel(const __grid_constant__ BeamArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int V = 16 / sizeof(T);  // elements of a load
     constexpr int kTile = kThreads * kVecs * V;
+    extern __shared__ __align__(16) char raw[];
+    Aside &aside = *reinterpret_cast<Aside *>(raw);
     __shared__ Picker s;
     __shared__ float2 red[kWarps];
+    const int warp = threadIdx.x >> 5;
     allow_next();
     const int row = blockIdx.y, part = blockIdx.x;
     const int b = (int)a.by_beams.div((uint32_t)row), k = row - b * a.beams;
@@ -264,10 +302,11 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
 
     float m = -INFINITY, sum = 0.f;
     uint4 nx[kVecs];
-    if (threadIdx.x == 0) s.count = 0;
+    if (threadIdx.x < kWarps) aside.count[threadIdx.x] = 0;
+    if (threadIdx.x == 0) aside.overflow = 0;
     if (first < last) fetch(first, nx);
-    bool overflow = false, grown = false;  // the same for the whole block
-    const int cut_at = 2 * a.n;
+    volatile uint32_t *const bound = &s.bound;
+    volatile int *const count = &aside.count[warp];
     for (int tile = first; tile < last; ++tile) {
         uint4 cur[kVecs];
 #pragma unroll
@@ -281,24 +320,27 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
             top[i] = largest<DT>(cur[i]);
             mx = fmaxf(mx, top[i]);
         }
-        const uint32_t best = ordered(mx);
-        if (tile == first) find_bound(best, a.n, s);
-        if (grown && !overflow) {
-            overflow = s.count > kMaxPicked;
-            if (!overflow) cut_picked(s, a.n);
-        }
-        int at = 0;
-        const uint32_t bound = max(s.bound, 1u);
-        if (best >= bound && !overflow) {
+        if (tile == first) find_bound(ordered(mx), a.n, s);
+        // (any finite logit while there are fewer than n)
+        const uint32_t reach = *bound;
+        const float low = reach ? from_ordered(reach) : -3.402823466e38f;
+        if (__any_sync(0xffffffffu, mx >= low)) {
 #pragma unroll
-            for (int i = 0; i < kVecs; ++i) {
-                if (ordered(top[i]) < bound) continue;
-                const uint32_t u[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const uint32_t o = ordered(element<DT>(u, e));
-                    if (o >= bound) at = pick(s, 0u, key_of(o, word_of(tile, i) + e));
+            for (int i = 0; i < kVecs; ++i)
+                if (top[i] >= low) {
+                    const int at = atomicAdd(&aside.count[warp], 1);
+                    if (at < kAside) {
+                        aside.data[warp][at] = cur[i];
+                        aside.word[warp][at] = word_of(tile, i);
+                    }
                 }
+            __syncwarp();
+            // after an overflow the list no longer matters: it is kept short
+            if (*count > kAsideLong) cut_aside<DT>(aside, warp, a.n, &s.bound);
+            if (*count > kAsideLong) {
+                __syncwarp();
+                *count = 0;
+                __syncwarp();
             }
         }
         // the thread's own maximum and sum; the maximum finite, so that -inf - m is -inf
@@ -331,7 +373,6 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
             }
         }
         sum += a0;
-        if (tile + 1 < last) grown = __syncthreads_or(at >= cut_at);
     }
 
 #pragma unroll
@@ -351,9 +392,24 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
         a.stat[at] = make_float2(top, all);
     }
 
+    // the bound again, among what was put aside (the barrier above is past every warp's last load)
+    uint32_t best = 0;
+    for (int i = threadIdx.x & 31; i < aside.count[warp]; i += 32) best = max(best, ordered(largest<DT>(aside.data[warp][i])));
+    find_bound(best, a.n, s);
+    const uint32_t reach = max(s.bound, 1u);
+    for (int i = threadIdx.x & 31; i < aside.count[warp]; i += 32) {
+        const uint4 d = aside.data[warp][i];
+        const int w = aside.word[warp][i];
+        const uint32_t u[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const uint32_t o = ordered(element<DT>(u, e));
+            if (o >= reach) pick(s, 0u, key_of(o, w + e));
+        }
+    }
     uint64_t *out = a.keys + at * a.n;
     auto emit = [&](int i, const Key &key) { out[i] = key.lo; };
-    if (!rank_picked(s, a.n, emit))
+    if (aside.overflow || !rank_picked(s, a.n, emit))
         rank_by_rounds(
             s, a.n,
             [&](const Key &under) {
@@ -437,8 +493,8 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const __grid_const
             emit);
 }
 
-// Parts of a row: one resident CTA for each of about four a SM, a tile at least
-// (batches past that stream whole rows).
+// Parts of a row: as many as three resident CTAs a SM allow, a tile at least
+// (larger batches stream whole rows).
 struct Plan {
     int parts, tiles;
 };
@@ -446,10 +502,19 @@ struct Plan {
 Plan plan(int64_t rows, int64_t vocab, int dtype) {
     const int64_t tile = (int64_t)kThreads * kVecs * (dtype == LQ_F32 ? 4 : 8);
     const int64_t all = ceil_div(vocab + 7, tile);  // a misaligned row starts up to 7 words in
-    int64_t parts = 148 * 4 / (rows < 1 ? 1 : rows);
+    int64_t parts = 148 * 3 / (rows < 1 ? 1 : rows);
     parts = parts < 1 ? 1 : parts > all ? all : parts;
     const int64_t tiles = ceil_div(all, parts);
     return Plan{(int)ceil_div(all, tiles), (int)tiles};
+}
+
+template <int DT>
+int launch_part(const BeamArgs &a, dim3 grid, cudaStream_t st) {
+    if (cudaFuncSetAttribute(beam_part_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Aside)) !=
+        cudaSuccess)
+        return LQ_ERR_CUDA;
+    beam_part_kernel<DT><<<grid, kThreads, sizeof(Aside), st>>>(a);
+    return check_launch();
 }
 
 bool beam_ok(int64_t batch, int64_t beams, int64_t vocab, int64_t n, int dtype) {
@@ -496,9 +561,9 @@ extern "C" int lq_beam_select(const void *logits, int dtype, int64_t batch, int6
     a.top_word = top_word;
     cudaStream_t st = as_stream(stream);
     const dim3 grid((unsigned)p.parts, (unsigned)(batch * beams));
-    if (dtype == LQ_F32) beam_part_kernel<LQ_F32><<<grid, kThreads, 0, st>>>(a);
-    else if (dtype == LQ_F16) beam_part_kernel<LQ_F16><<<grid, kThreads, 0, st>>>(a);
-    else beam_part_kernel<LQ_BF16><<<grid, kThreads, 0, st>>>(a);
-    if (check_launch() != LQ_OK) return LQ_ERR_CUDA;
+    const int status = dtype == LQ_F32   ? launch_part<LQ_F32>(a, grid, st)
+                       : dtype == LQ_F16 ? launch_part<LQ_F16>(a, grid, st)
+                                         : launch_part<LQ_BF16>(a, grid, st);
+    if (status != LQ_OK) return status;
     return launch_overlapped(beam_merge_kernel, dim3((unsigned)batch), kThreads, 0, st, a);
 }
