@@ -510,14 +510,12 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
         for (int j = set; j < n_tiles; j += X::kDecodeSets) {
             const int s = j & 1, stage = j % X::kStages;
             const uint32_t from = stages + stage * X::kStageBytes + dt * 16;
-            if (j >= 2) {
-                wait(sm.k_free[s], (j >> 1) - 1);
-                wait(sm.v_free[s], (j >> 1) - 1);
-            }
+            if (j >= 2) wait(sm.k_free[s], (j >> 1) - 1);
             wait(sm.stage_full[stage], j / X::kStages);
             put(sk + s * X::kTileBytes, from);
             publish_smem();
             arrive_warp(smem_u32(&sm.k_full[s]));
+            if (j >= 2) wait(sm.v_free[s], (j >> 1) - 1);
             put(sv + s * X::kTileBytes, from + X::kWordBytes);
             publish_smem();
             __syncwarp();
