@@ -239,6 +239,61 @@ def test_attention_matches_float64(P, lens, H, G, T, D, page, dtype, mask):
     _check(again, lse, o.double().cpu().numpy(), lse.double().cpu().numpy())
 
 
+def _ref_gpu(q, codes, scales, table, lens, mask, scale):
+    """_ref on the GPU in float64, for batches too large for the host: K and V of every sequence at the longest length."""
+    B, Hq, T, D = q.shape
+    H, page = codes.shape[2], codes.shape[3]
+    n = table.shape[1] * page
+    shift = torch.tensor([27, 23, 19, 15, 11, 7, 3], device="cuda")
+    pg = table.clamp(min=0).long()
+    w = codes[pg].long() & 0xFFFFFFFF
+    u = (w[..., None] >> shift) & 15
+    last = 2 * (w & 7) + u.sum(-1) % 2
+    pts = torch.cat([u, last[..., None]], -1).double() - 8 + 0.5 * (w >> 31)[..., None]
+    kv = (pts.flatten(-2) * scales[pg].double()[..., None]).nan_to_num(0)  # (B, width, 2, H, page, D)
+    k, v = kv.permute(2, 0, 3, 1, 4, 5).reshape(2, B, H, 1, n, D)
+    j = torch.arange(n, device="cuda")[None, None] - (lens.long()[:, None, None] - T)
+    see = (j < 0).expand(B, T, n).clone()
+    t = torch.arange(T, device="cuda")[None, :, None]
+    drafts = (j >= 0) & (j < T)
+    if mask is None:
+        see |= drafts & (j <= t)
+    else:
+        see |= drafts & mask.expand(B, T, T).gather(2, j.clamp(0, T - 1).expand(B, T, n))
+    x = q.double().view(B, H, Hq // H * T, D) @ k.squeeze(2).transpose(2, 3) * scale
+    x = x.view(B, H, Hq // H, T, n).masked_fill(~see[:, None, None], float("-inf"))
+    lse = torch.logsumexp(x, -1)
+    p = torch.exp(x - torch.where(torch.isinf(lse), 0.0, lse)[..., None])
+    o = (p.view(B, H, -1, n) @ v.squeeze(2)).view(B, Hq, T, D)
+    return o.cpu().numpy(), lse.view(B, Hq, T).cpu().numpy()
+
+
+# enough (sequence, head) pairs that a CTA walks many tiles: every kernel's pipeline goes round its buffers
+@pytest.mark.parametrize("G,T,D,page,dtype", [
+    (4, 1, 128, 64, torch.bfloat16), (8, 1, 64, 16, torch.float16),                     # up to 8 rows
+    (4, 4, 128, 32, torch.float16), (3, 5, 64, 64, torch.bfloat16),                     # 16
+    (7, 4, 128, 128, torch.bfloat16), (2, 16, 64, 32, torch.float16),                   # 32
+    (4, 13, 128, 16, torch.float16), (8, 8, 64, 256, torch.bfloat16), (4, 13, 128, 256, torch.bfloat16),  # 64
+    (5, 33, 128, 64, torch.float16),                                                    # more than one CTA's rows
+])
+def test_attention_many_tiles(P, G, T, D, page, dtype):
+    g = torch.Generator(device="cuda").manual_seed(G * 100 + T)
+    B, H = 75, 8
+    rng = np.random.default_rng(T)
+    lens = [int(x) for x in rng.integers(0, 1700, B)]
+    lens[0], lens[1], lens[2], lens[3] = 1700, 0, 1, 1664
+    codes, scales, table, ln = _pool(P, g, lens, H, D, page, spread=1.0, dtype=dtype)
+    q = (2 * torch.randn(B, H * G, T, D, device="cuda", generator=g)).to(dtype)
+    m = _tree(T, T, B) if T > 1 else None
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    o, lse = P.tree_attention(q, codes, scales, table, ln, m, return_lse=True, err=err)
+    assert int(err.item()) == 0
+    ro, rl = _ref_gpu(q, codes, scales, table, ln, m, 1 / math.sqrt(D))
+    _check(o, lse, ro, rl)
+    for _ in range(3):  # nothing in the result depends on timing
+        assert torch.equal(o, P.tree_attention(q, codes, scales, table, ln, m))
+
+
 @pytest.mark.parametrize("T", [2, 40])
 def test_attention_rows_that_see_nothing(P, T):
     """No context and an empty mask row: o = 0, lse = -inf; other rows are unaffected."""
