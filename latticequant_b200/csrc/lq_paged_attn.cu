@@ -18,8 +18,8 @@
 //   x = s * log2(e) * sm_scale * ks + log2(vs),  w = 2^(x - M),
 //   o += w * point,  l += w / vs
 // so the fp16 weights w stay within 2^15 whatever the scales are.  M is a
-// reference, not the running maximum: it moves (to the maximum) only when an
-// x exceeds it by 15, which a warp vote finds; the statistics are then
+// reference, not the running maximum: it moves (to the maximum less 4) only
+// when an x exceeds it by 15, which a warp vote finds; the statistics are then
 // rescaled.  W^T reaches its B registers with one 8x8 transpose per 8
 // tokens; V's A registers pair two tokens' decoded channels by byte permutes.
 #include "lq_paged.cuh"
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
                     float mx = fmaxf(s[n][c], s[n][2 + c]);
 #pragma unroll
                     for (int off = 4; off <= 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                    const float mn = fmaxf(m[n][c], mx);
+                    const float mn = fmaxf(m[n][c], mx - kRefBelow);
                     const float f = exp2f(m[n][c] - mn);
                     m[n][c] = mn;
                     l[n][c] *= f;

@@ -31,10 +31,11 @@ struct PagedAttnArgs {
     uint32_t *err;
 };
 
-// The reference M of the base-2 weights 2^(x - M): "none yet", and how far an x
-// may exceed it (fp16 holds 2^15; a weight under 2^-14 of the reference loses
-// at most 2^-25 of it).  It is put at a maximum, so it rarely moves again.
-constexpr float kNoRef = -1e30f, kRefSlack = 15.f;
+// The reference M of the base-2 weights 2^(x - M): "none yet", how far an x
+// may exceed it (fp16 holds 2^15), and how far below a maximum it is put: the
+// 2^4 keep weights down to 2^-18 of the largest out of fp16's subnormals, and
+// the 2^11 left let the maximum grow before M has to move again.
+constexpr float kNoRef = -1e30f, kRefSlack = 15.f, kRefBelow = 4.f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

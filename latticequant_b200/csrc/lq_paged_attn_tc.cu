@@ -187,7 +187,7 @@ struct Shape {
     static constexpr int kOperands = 4 * kTileBytes + kN * D * 2 + kSets * kHalfBytes;
     // a stage: the code words of K and V and the scales of K and V of 128 tokens
     static constexpr int kWordBytes = kTok * D / 2, kStageBytes = 2 * kWordBytes + 2 * kTok * 4;
-    static constexpr int kStages = 3;
+    static constexpr int kStages = D == 128 ? 3 : 6;
 };
 
 // Shared memory after the 1024-byte aligned operands and the stages.
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
                 if (tl < C) {
                     const int n = col0 + tl;
                     const float top = fmaxf(fmaxf(red[0][n], red[1][n]), fmaxf(red[2][n], red[3][n]));
-                    const float m = -minus_m[tl], next = fmaxf(m, top);
+                    const float m = -minus_m[tl], next = fmaxf(m, top - kRefBelow);
                     f[tl] = ex2(m - next);
                     minus_m[tl] = -next;
                 }
