@@ -566,3 +566,27 @@ def test_accept_matches_loops(P, page, D, H):
         out = P.accept_tokens(codes, scales, *args, T, torch.from_numpy(accepted).cuda(), err)
         assert int(err.item()) == _lib.EF_PAGE and int(out[0]) == lens[0]
         assert torch.equal(codes, c0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_append_equals_the_frameworks_search_at_its_ties(P, dtype):
+    """Values on the lattice's decision surfaces (quarter steps of the scale, repeated magnitudes), where the
+    search's short form hands over to the long one, and a million blocks of ordinary values."""
+    from latticequant_b200.core import e8_quantizer
+
+    g = torch.Generator(device="cuda").manual_seed(11)
+    n, H, D = 4096, 2, 128
+    # a first channel of 7 - 1/64 makes the scale 1 up to a rounding, so the rest are exact steps of it
+    x = torch.randint(-27, 28, (n, H, D), device="cuda", generator=g).float() / 4
+    x[..., 0] = 7 - 1 / 64
+    y = torch.randn(n, H, D, device="cuda", generator=g)
+    y[: n // 2, :, 8:16] = y[: n // 2, :, 8:9] * torch.where(torch.rand(n // 2, H, 8, device="cuda", generator=g) < 0.5, -1, 1)
+    for v in (x.to(dtype), y.to(dtype)):
+        codes, scales, _ = P.empty_pool(1, n // 64, H, D, 64)
+        k, _ = P.append(codes[0], scales[0], v, v, torch.arange(n, device="cuda"), dequantised=True)
+        amax = v.float().abs().amax(-1)
+        s = amax * float(np.float32(1) / BOUND)
+        q = e8_quantizer.encode_e8((v.float() / s[..., None]).reshape(-1, 8)).view(n, H, D)
+        assert torch.equal(k, (q * s[..., None]).to(dtype))
+        stored = _values(codes[0, :, 0], scales[0, :, 0]).transpose(0, 2, 1, 3).reshape(n, H, D)
+        assert np.array_equal(stored, q.double().cpu().numpy() * s[..., None].double().cpu().numpy())
