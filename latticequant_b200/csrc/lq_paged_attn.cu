@@ -455,11 +455,16 @@ int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st
     return launch_overlapped(paged_combine_kernel<BF16, D>, dim3((unsigned)ceil_div(n, 4)), 128, 0, st, a, n);
 }
 
-// Rows of a CTA and tokens of a split: enough CTAs for about four rounds of
-// the GPU, chunks of a tile of tokens at least.  Up to kClusterMax splits of
-// the few-rows kernel form a cluster and join over its shared memory, which
-// spares the second launch and the workspace; short contexts take fewer
-// splits for it than would fill the GPU.
+// Rows of a CTA and tokens of a split.  The CTAs of a call come in rounds of
+// as many as the GPU holds, so the number of splits is the one whose rounds
+// times a CTA's time (its tiles, and kStartTiles tiles' worth of start and end)
+// is smallest, among those that fill one round where the tokens allow chunks
+// of kShortest tiles.  (Tree of 13 over 16 ragged sequences, up to 8,190
+// tokens: 2 splits 59.6 us, 3 72.6, 5 67.9; tree of 64 over 4 x 32,768 tokens:
+// 5 splits 308 us, 6 326, 4 371.)
+// Up to kClusterMax splits of the few-rows kernel form a cluster and join over
+// its shared memory, which spares the second launch and the workspace; short
+// contexts take fewer splits for it than would fill the GPU.
 struct Plan {
     int tile;
     int64_t chunk;
@@ -467,20 +472,33 @@ struct Plan {
     bool clustered;
 };
 constexpr int64_t kClusterMax = 8, kClusterTokens = 256;  // splits, and the chunk up to which 8 of them are enough
+constexpr int64_t kStartTiles = 3, kShortest = 4, kMostSplits = 512;
 
 Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
     Plan p;
     p.tile = rows <= kFewRows ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    const int64_t least = p.tile == 8 ? 64 : 128;
+    const int64_t tile_tokens = p.tile == 8 ? 64 : 128, slots = 148 * (p.tile == 8 ? 4 : 1);
     const int64_t units = batch * n_heads * ceil_div(rows, p.tile);  // CTAs without a split
-    const int64_t want = ceil_div((int64_t)148 * (p.tile == 8 ? 16 : 4), units);
-    const int64_t tokens = max_len < 1 ? 1 : max_len;
-    p.chunk = ceil_div(ceil_div(tokens, want), least) * least;
+    const int64_t tokens = max_len < 1 ? 1 : max_len, tiles = ceil_div(tokens, tile_tokens);
+    int64_t best = 0, best_cost = INT64_MAX;
+    for (int64_t s = 1; s <= tiles && s <= kMostSplits; ++s) {
+        const int64_t each = ceil_div(tiles, s);
+        if (ceil_div(tiles, each) != s) continue;  // no such split
+        if (units * s < slots && each > kShortest && s < kMostSplits && s < tiles) continue;
+        const int64_t cost = ceil_div(units * s, slots) * (each + kStartTiles);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = each;
+        }
+        if (units * s > 16 * slots) break;  // only more starts from here
+    }
+    if (best == 0) best = ceil_div(tiles, kMostSplits);
+    p.chunk = best * tile_tokens;
     p.splits = (uint32_t)ceil_div(tokens, p.chunk);
     p.clustered = p.tile == 8 && p.splits > 1 && (p.splits <= kClusterMax || tokens <= kClusterMax * kClusterTokens);
     if (p.clustered) {  // 2, 4 or 8 CTAs (the last may find nothing to do)
         p.splits = p.splits <= 2 ? 2 : p.splits <= 4 ? 4 : 8;
-        p.chunk = ceil_div(ceil_div(tokens, p.splits), least) * least;
+        p.chunk = ceil_div(ceil_div(tokens, p.splits), tile_tokens) * tile_tokens;
     }
     return p;
 }

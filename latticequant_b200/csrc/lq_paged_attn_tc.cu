@@ -166,6 +166,26 @@ __device__ __forceinline__ bool any128(int id, bool x) {
     return r != 0;
 }
 
+// C values of every lane folded over the warp: lane i ends with value i / (32 / C).  Each step halves the
+// values that a lane carries and sends the other half, so C shuffles do for C values.
+template <int C, class Op>
+__device__ __forceinline__ float fold(float (&v)[C], Op op) {
+    const int lane = threadIdx.x & 31;
+    int off = 16;
+#pragma unroll
+    for (int n = C / 2; n >= 1; n /= 2, off /= 2) {
+        const bool up = lane & off;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float keep = up ? v[i + n] : v[i], send = up ? v[i] : v[i + n];
+            v[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, off));
+        }
+    }
+#pragma unroll
+    for (; off >= 1; off /= 2) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], off));
+    return v[0];
+}
+
 // The kernel for D channels and up to COLS query rows a CTA.
 template <int D, int COLS>
 struct Shape {
@@ -243,13 +263,13 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
     }
     const int n_tiles = (last - first + kTok - 1) / kTok;
 
-    if (warp == 0) {
+    if (warp == X::kIssue) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
                      "r"(X::kTmem)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (tid == 0) {
+    if (tid == 32 * (X::kIssue + 1)) {
         auto init = [](uint64_t &bar, uint32_t n) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&bar)), "r"(n) : "memory");
         };
@@ -275,6 +295,25 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
     }
     for (int n = tid; n < X::kSets * N; n += kThreads) sm.minus_m[n / N][n % N] = -kNoRef;
 
+    // Q's loads are on their way over the barrier, and the producer's first pages
+    constexpr int kLoaders = 32 * X::kSoftmax, kChunks = N * W;  // 16-byte chunks of Q
+    constexpr int kQ = (kChunks + kLoaders - 1) / kLoaders;
+    uint4 q[kQ];
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+        const int e = tid + i * kLoaders, n = e / W, c = e % W;
+        q[i] = make_uint4(0, 0, 0, 0);
+        if (tid < kLoaders && e < kChunks && n < live) {
+            const uint32_t r = row0 + n, qt = a.by_group.div(r), qh = h * a.group + (r - qt * a.group);
+            q[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
+                                                         qh * a.q_stride_h + qt * a.q_stride_t) + c);
+        }
+    }
+    const int seg_log2 = min((int)a.page_log2, 7), segs = kTok >> seg_log2;  // runs of a tile's rows in one page
+    const int32_t *table = a.table + b * a.table_stride;
+    auto entry_of = [&](int tok) { return lane < segs && tok < last ? __ldg(table + (tok >> a.page_log2)) : 0; };
+    int tok_p = first + (lane << seg_log2), page = 0;
+    if (warp == X::kIssue + 2) page = entry_of(tok_p);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -284,21 +323,8 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
     if (warp < X::kSoftmax) {
         // ---- softmax: token tl (a TMEM lane), columns col0.., every kSets-th tile
         // Q: fp16 rows in the decoded blocks' channel order; rows past the last are zero
-        constexpr int kLoaders = 32 * X::kSoftmax, kChunks = N * W;  // 16-byte chunks
-        constexpr int kQ = (kChunks + kLoaders - 1) / kLoaders;
         float qk = a.qk_log2 * kCodeUnit;
         {
-            uint4 q[kQ];
-    #pragma unroll
-            for (int i = 0; i < kQ; ++i) {
-                const int e = tid + i * kLoaders, n = e / W, c = e % W;
-                q[i] = make_uint4(0, 0, 0, 0);
-                if (e < kChunks && n < live) {
-                    const uint32_t r = row0 + n, qt = a.by_group.div(r), qh = h * a.group + (r - qt * a.group);
-                    q[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
-                                                                 qh * a.q_stride_h + qt * a.q_stride_t) + c);
-                }
-            }
             if constexpr (BF16) {  // a power of two for all rows puts the largest finite value in [2^10, 2^11)
                 uint32_t e = 27;   // (at least 2^-100)
     #pragma unroll
@@ -339,7 +365,6 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
         float *const minus_m = sm.minus_m[set] + col0, *const f = sm.f[set] + col0;
         float(*const red)[N] = sm.red[set];
         const uint32_t my_p = sp + set * kHalfBytes + tl * 128;
-        const int seg_log2 = min((int)a.page_log2, 7);
         unsigned long long l[C / 2];  // of two columns each, as packed fp32
 #pragma unroll
         for (int c = 0; c < C / 2; ++c) l[c] = 0;
@@ -390,13 +415,8 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
             if (move) {
                 // the tile's column maxima move the references; l and O follow
                 scores();
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    float top = x[c];
-#pragma unroll
-                    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    if (lane == 0) red[warp & 3][col0 + c] = top;
-                }
+                const float warp_top = fold(x, [](float p, float q) { return fmaxf(p, q); });
+                if (lane % (32 / C) == 0) red[warp & 3][col0 + lane / (32 / C)] = warp_top;
                 sync128(vote);
                 if (tl < C) {
                     const int n = col0 + tl;
@@ -406,6 +426,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
                     minus_m[tl] = -next;
                 }
                 sync128(vote);
+                scores();
                 less_reference();
 #pragma unroll
                 for (int c = 0; c < C; c += 2) l[c / 2] = f2_mul(l[c / 2], f2_pack(f[c], f[c + 1]));
@@ -441,15 +462,11 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
         // denominators over the 128 tokens, then O: a lane is a channel
         if (done > 0) wait(sm.p_free[set], done - 1);
         tmem_fence_after();
+        float sums[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float l0, l1;
-            f2_unpack(l[c / 2], l0, l1);
-            float sum = c & 1 ? l1 : l0;
-#pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) red[warp & 3][col0 + c] = sum;
-        }
+        for (int c = 0; c < C; c += 2) f2_unpack(l[c / 2], sums[c], sums[c + 1]);
+        const float sum = fold(sums, [](float p, float q) { return p + q; });
+        if (lane % (32 / C) == 0) red[warp & 3][col0 + lane / (32 / C)] = sum;
         float o[C];
         tmem_load<C>(o_at, o);
         tmem_fence_before();
@@ -568,14 +585,12 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
             }
         } else if (issuer == 2) {
             // lane i < segs copies the tile's i-th run of rows that lie in one page
-            const int seg_log2 = min((int)a.page_log2, 7), segs = kTok >> seg_log2;
-            const int32_t *table = a.table + b * a.table_stride;
             const int64_t side = (int64_t)a.n_heads << a.page_log2;
             const uint32_t *kbase = a.codes + ((int64_t)h << a.page_log2) * W;
             const float *sbase = a.scales + ((int64_t)h << a.page_log2);
-            auto entry_of = [&](int tok) { return lane < segs && tok < last ? __ldg(table + (tok >> a.page_log2)) : 0; };
-            int tok = first + (lane << seg_log2), page = entry_of(tok), stage = 0;
-            for (int j = 0; j < n_tiles; ++j, tok += kTok) {
+            int stage = 0;
+            for (int j = 0; j < n_tiles; ++j, tok_p += kTok) {
+                const int tok = tok_p;
                 const bool mine = lane < segs && tok < last, bad = mine && (uint32_t)page >= (uint32_t)a.n_pages;
                 const int64_t row = 2 * side * (bad ? 0 : page) + (tok & ((1 << a.page_log2) - 1));
                 page = entry_of(tok + kTok);
@@ -602,7 +617,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
     }
     if (!wait.alive) raise_flag(a.err, LQ_EF_TIMEOUT);
     __syncthreads();
-    if (warp == 0)
+    if (warp == X::kIssue)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(ts), "r"(X::kTmem) : "memory");
 }
 
