@@ -458,10 +458,11 @@ int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st
 // Rows of a CTA and tokens of a split.  The CTAs of a call come in rounds of
 // as many as the GPU holds, so the number of splits is the one whose rounds
 // times a CTA's time (its tiles, and kStartTiles tiles' worth of start and end)
-// is smallest, among those that fill one round where the tokens allow chunks
-// of kShortest tiles.  (Tree of 13 over 16 ragged sequences, up to 8,190
-// tokens: 2 splits 59.6 us, 3 72.6, 5 67.9; tree of 64 over 4 x 32,768 tokens:
-// 5 splits 308 us, 6 326, 4 371.)
+// is smallest, among those that fill two rounds where the tokens allow chunks
+// of kShortest tiles, for lengths that differ from the bound.  (Tree of 13 over
+// 16 sequences of up to 8,190 tokens, mean over eight draws of their lengths:
+// no such floor 95.8 us, one round 81.2, two 80.7, three 81.3, five 93.9; tree
+// of 64 over 4 x 32,768 tokens: 5 splits 308 us, 6 326, 4 371.)
 // Up to kClusterMax splits of the few-rows kernel form a cluster and join over
 // its shared memory, which spares the second launch and the workspace; short
 // contexts take fewer splits for it than would fill the GPU.
@@ -484,7 +485,7 @@ Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
     for (int64_t s = 1; s <= tiles && s <= kMostSplits; ++s) {
         const int64_t each = ceil_div(tiles, s);
         if (ceil_div(tiles, each) != s) continue;  // no such split
-        if (units * s < slots && each > kShortest && s < kMostSplits && s < tiles) continue;
+        if (units * s < 2 * slots && each > kShortest && s < kMostSplits && s < tiles) continue;
         const int64_t cost = ceil_div(units * s, slots) * (each + kStartTiles);
         if (cost < best_cost) {
             best_cost = cost;
