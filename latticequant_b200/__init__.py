@@ -8,6 +8,7 @@ dequantisation / fused decode attention, as hand-written CUDA behind a C ABI
                                             compact_storage, triton_dequant, pipeline
   latticequant_b200.llm.compressed_kv_cache CompressedKVCache
   latticequant_b200.allocation.eval_alloc   VariableRateKVCache
+  latticequant_b200.llm.paged_cache         PagedKVCache (search decoding; paged, beam below it)
 
 There is no CPU fallback: every compute call runs the CUDA library.
 """

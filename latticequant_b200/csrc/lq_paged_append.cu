@@ -13,7 +13,10 @@
 // the framework's own (e8_nearest_symbols), bit for bit the torch form.
 //
 // One thread per block of 8 channels: a token-head is 8 or 16 neighbouring
-// lanes, its amax a shuffle maximum.
+// lanes, its amax a shuffle maximum.  What bounds it is instruction issue, most
+// of it the search (480 instructions a thread, 76% of issue slots): 16,411
+// tokens of 4 heads of 128 in fp16 with their values returned take 35 us, 2.2
+// TB/s.
 #include "lq_paged.cuh"
 
 namespace lq {

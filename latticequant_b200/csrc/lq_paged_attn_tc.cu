@@ -22,7 +22,10 @@
 // sets of softmax warps take the tiles in turn, each with references,
 // denominators and an O of its own that are joined at the end, and with up to
 // 16 two sets of decoders do.
-// so copying, decoding, the tensor cores and the exponentials overlap.
+// so copying, decoding, the tensor cores and the exponentials overlap.  64
+// positions over 4 sequences of 32,768 tokens (448 rows of 4 KV heads of 128):
+// 308 us, 390 TFLOP/s; mma.sync from registers took 749, and this kernel with
+// one barrier-synchronised part for all warps 413.
 //
 // M is a reference per row, moved only when an x exceeds it by kRefSlack,
 // which a vote of the 128 threads finds; O is then rescaled in TMEM.
