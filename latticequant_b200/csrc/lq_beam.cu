@@ -544,6 +544,7 @@ extern "C" int lq_beam_select(const void *logits, int dtype, int64_t batch, int6
     if (!beam_ok(batch, beams, vocab, n, dtype)) return LQ_ERR_INVALID;
     if (batch == 0) return LQ_OK;
     if (!logits || !scores || !top_score || !top_beam || !top_word || !workspace) return LQ_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 7) != 0) return LQ_ERR_INVALID;
     if (workspace_bytes < lq_beam_select_workspace(dtype, batch, beams, vocab, n)) return LQ_ERR_CAPACITY;
     const Plan p = plan(batch * beams, vocab, dtype);
     BeamArgs a{};

@@ -9,7 +9,7 @@
 // dequantised buffer (llm/compressed_kv_cache.py:342-395).
 //
 // Mathematics.  A query row r = t * G + g; the tile of a warp is 16 tokens by
-// 8 * NT rows.  Scores S = K Q^T put tokens on the rows of the MMA, so a
+// 8 rows.  Scores S = K Q^T put tokens on the rows of the MMA, so a
 // lane's A registers are whole code words of "its" two tokens, decoded in
 // registers to fp16, which holds every point exactly.  A bf16 query becomes
 // fp16 times a power of two of its row (its largest value then lies in
@@ -24,11 +24,11 @@
 // tokens; V's A registers pair two tokens' decoded channels by byte permutes.
 //
 // Registers feed the MMAs, no shared memory: with 8 rows a tile's MMAs are few,
-// and what bounds the kernel is the decode's instructions (70% of issue slots,
-// the integer ALU over half).  The next tile's words load into the registers
+// and what bounds the kernel is issue, most of it the decode (488 instructions a
+// warp and tile of 16 tokens; 70% of issue slots, the integer ALU over half).  The next tile's words load into the registers
 // that this tile's were decoded from.  32 sequences of 16,384 tokens, 8 KV
-// heads of 128, 4 query heads each: 196 us, 2.9 TB/s (the tcgen05 kernel, with
-// 8 of its 16 columns used, takes 247); 1 sequence of 777 tokens: 6.0 us.
+// heads of 128, 4 query heads each: 194-198 us, 2.9 TB/s; 1 sequence of 777
+// tokens: 6.0 us.
 #include "lq_paged.cuh"
 #include "lq_paged_attn.cuh"
 
@@ -36,7 +36,7 @@ namespace lq {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int64_t kFewRows = 8;  // up to here this kernel, above lq_paged_attn_tc.cu
+constexpr int kTileRows = 8;  // query rows of a CTA
 
 __device__ __forceinline__ void mma_16816(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -125,101 +125,90 @@ __device__ __forceinline__ void load_v(const TileAt &at, uint32_t g, uint32_t t,
 }
 
 // v[block][half]: tokens 2t, 2t+1 (+ 8 half) of this lane's blocks
-template <int D, int NT, int S>
-__device__ __forceinline__ void pv_step(const TokenPair v[D / 64][2], const uint32_t (*p)[2], float (*o)[NT][4]) {
+template <int D, int S>
+__device__ __forceinline__ void pv_step(const TokenPair v[D / 64][2], const uint32_t (&p)[2], float (*o)[4]) {
     if constexpr (D == 128) {
         uint32_t a[4], b[4];  // [block + 2 half] of the pair's two channels
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
             for (int half = 0; half < 2; ++half) decode_pair<S>(v[blk][half], a[blk + 2 * half], b[blk + 2 * half]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            mma_16816(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
-            mma_16816(o[4 + S][n], b[0], b[1], b[2], b[3], p[n][0], p[n][1]);
-        }
+        mma_16816(o[S], a[0], a[1], a[2], a[3], p[0], p[1]);
+        mma_16816(o[4 + S], b[0], b[1], b[2], b[3], p[0], p[1]);
     } else {
         uint32_t a[4];  // one block: its two channels are the MMA's two row groups
 #pragma unroll
         for (int half = 0; half < 2; ++half) decode_pair<S>(v[0][half], a[2 * half], a[1 + 2 * half]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_16816(o[S][n], a[0], a[1], a[2], a[3], p[n][0], p[n][1]);
+        mma_16816(o[S], a[0], a[1], a[2], a[3], p[0], p[1]);
     }
 }
 
 // grid (splits, n_heads * row tiles, batch); a CTA's warps take the 16-token
 // tiles of its chunk in turn.
-template <bool BF16, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+template <bool BF16, int D>
+__global__ void __launch_bounds__(32 * kWarps, 4) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int KW = D / 32, VW = D / 64, W = D / 8, MT = D / 16;
-    constexpr int ROWS = 8 * NT;
-    extern __shared__ __align__(16) float sm[];  // [warps][ROWS][D + 4]
+    extern __shared__ __align__(16) float sm[];  // [warps][kTileRows][D + 4]
     const int warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t b = blockIdx.z, rt = blockIdx.y / a.n_heads, h = blockIdx.y - rt * a.n_heads;
-    const uint32_t row0 = rt * ROWS;
+    const uint32_t row0 = rt * kTileRows;
     // positions fit 32 bits: a table is at most 2^20 pages of 2^8 tokens
     const int len = (int)paged_len(a, b);
     const int first = (int)(blockIdx.x * a.chunk), last = (int)min(first + a.chunk, (int64_t)len);
     const int drafts = len - (int)a.T;  // position of draft 0
     if (len < a.lens[b] && (blockIdx.x | blockIdx.y | threadIdx.x) == 0) raise_flag(a.err, LQ_EF_PAGE);
 
-    // Q's B registers: row n = lane / 4 of each 8-row group, this lane's blocks
-    uint32_t qf[NT][KW * 4];
-    float qk[NT][2];  // what a score of the lane's rows 2t, 2t + 1 is multiplied by
+    // Q's B registers: row lane / 4, this lane's blocks
+    uint32_t qf[KW * 4];
+    float qk[2];  // what a score of the lane's rows 2t, 2t + 1 is multiplied by
+    const uint32_t r = row0 + g;
+    const bool in = r < a.rows;
+    const uint32_t qt = in ? a.by_group.div(r) : 0, qh = h * a.group + (in ? r - qt * a.group : 0);
+    const uint4 *qp = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
+                                                      qh * a.q_stride_h + qt * a.q_stride_t);
+    uint4 u[KW];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const uint32_t r = row0 + 8 * n + g;
-        const bool in = r < a.rows;
-        const uint32_t qt = in ? a.by_group.div(r) : 0, qh = h * a.group + (in ? r - qt * a.group : 0);
-        const uint4 *qp = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + b * a.q_stride_b +
-                                                          qh * a.q_stride_h + qt * a.q_stride_t);
-        uint4 u[KW];
+    for (int j = 0; j < KW; ++j) u[j] = in ? __ldg(qp + t * KW + j) : make_uint4(0, 0, 0, 0);
+    float back = a.qk_log2 * kCodeUnit;
+    if constexpr (BF16) {
+        uint32_t e = 0;  // the row's largest finite exponent
 #pragma unroll
-        for (int j = 0; j < KW; ++j) u[j] = in ? __ldg(qp + t * KW + j) : make_uint4(0, 0, 0, 0);
-        float back = a.qk_log2 * kCodeUnit;
-        if constexpr (BF16) {
-            uint32_t e = 0;  // the row's largest finite exponent
+        for (int j = 0; j < KW; ++j) {
+            const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
-            for (int j = 0; j < KW; ++j) {
-                const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t lo = w[i] >> 7 & 0xffu, hi = w[i] >> 23 & 0xffu;
-                    e = max(e, max(lo == 0xffu ? 0u : lo, hi == 0xffu ? 0u : hi));
-                }
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t lo = w[i] >> 7 & 0xffu, hi = w[i] >> 23 & 0xffu;
+                e = max(e, max(lo == 0xffu ? 0u : lo, hi == 0xffu ? 0u : hi));
             }
-            e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
-            e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
-            e = max(e, 27u);  // rows under 2^-100 count as 2^-100
-            const float f = __uint_as_float((264u - e) << 23);  // 2^(10 - (e - 127))
-            back *= __uint_as_float((e - 10u) << 23);           // 1 / f
-#pragma unroll
-            for (int j = 0; j < KW; ++j)
-                u[j] = make_uint4(bf16_to_f16(u[j].x, f), bf16_to_f16(u[j].y, f), bf16_to_f16(u[j].z, f),
-                                  bf16_to_f16(u[j].w, f));
         }
+        e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
+        e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
+        e = max(e, 27u);  // rows under 2^-100 count as 2^-100
+        const float f = __uint_as_float((264u - e) << 23);  // 2^(10 - (e - 127))
+        back *= __uint_as_float((e - 10u) << 23);           // 1 / f
 #pragma unroll
-        for (int c = 0; c < 2; ++c) qk[n][c] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + c));
+        for (int j = 0; j < KW; ++j)
+            u[j] = make_uint4(bf16_to_f16(u[j].x, f), bf16_to_f16(u[j].y, f), bf16_to_f16(u[j].z, f),
+                              bf16_to_f16(u[j].w, f));
+    }
 #pragma unroll
-        for (int j = 0; j < KW; ++j) {  // decode_block's pair s: channels 7 - s, 3 - s
-            qf[n][4 * j + 0] = __byte_perm(u[j].w, u[j].y, 0x7632);
-            qf[n][4 * j + 1] = __byte_perm(u[j].w, u[j].y, 0x5410);
-            qf[n][4 * j + 2] = __byte_perm(u[j].z, u[j].x, 0x7632);
-            qf[n][4 * j + 3] = __byte_perm(u[j].z, u[j].x, 0x5410);
-        }
+    for (int c = 0; c < 2; ++c) qk[c] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + c));
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {  // decode_block's pair s: channels 7 - s, 3 - s
+        qf[4 * j + 0] = __byte_perm(u[j].w, u[j].y, 0x7632);
+        qf[4 * j + 1] = __byte_perm(u[j].w, u[j].y, 0x5410);
+        qf[4 * j + 2] = __byte_perm(u[j].z, u[j].x, 0x7632);
+        qf[4 * j + 3] = __byte_perm(u[j].z, u[j].x, 0x5410);
     }
 
-    float o[MT][NT][4], l[NT][2], m[NT][2];
+    float o[MT][4], l[2], m[2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[i][n][c] = 0.f;
-        l[n][0] = l[n][1] = 0.f;
-        m[n][0] = m[n][1] = kNoRef;
-    }
+        for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+    l[0] = l[1] = 0.f;
+    m[0] = m[1] = kNoRef;
 
     const int32_t *table = a.table + b * a.table_stride;
     const uint32_t *kbase = a.codes + ((int64_t)h << a.page_log2) * W;
@@ -251,19 +240,14 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
         page = page_nx;
         page_nx = page_of(tok + 2 * kStep);
 
-        float s[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        float s[4] = {};
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
             uint32_t k0[4], k1[4];
             decode_block(x.k[0][j], k0);
             decode_block(x.k[1][j], k1);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mma_16816(s[n], k0[0], k1[0], k0[1], k1[1], qf[n][4 * j], qf[n][4 * j + 1]);
-                mma_16816(s[n], k0[2], k1[2], k0[3], k1[3], qf[n][4 * j + 2], qf[n][4 * j + 3]);
-            }
+            mma_16816(s, k0[0], k1[0], k0[1], k1[1], qf[4 * j], qf[4 * j + 1]);
+            mma_16816(s, k0[2], k1[2], k0[3], k1[3], qf[4 * j + 2], qf[4 * j + 3]);
         }
 
         if (more) load_k<D>(next, g, t, x);
@@ -274,11 +258,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
         for (int r = 0; r < 2; ++r) {
             const float lv = lg2(x.vs[r]);
             rvs[r] = rcp(x.vs[r]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                s[n][2 * r] = fmaf(s[n][2 * r], x.ks[r] * qk[n][0], lv);
-                s[n][2 * r + 1] = fmaf(s[n][2 * r + 1], x.ks[r] * qk[n][1], lv);
-            }
+            s[2 * r] = fmaf(s[2 * r], x.ks[r] * qk[0], lv);
+            s[2 * r + 1] = fmaf(s[2 * r + 1], x.ks[r] * qk[1], lv);
         }
         if (more) load_scales<D>(next, g, x);
         if (tok + 16 > drafts || bad) {  // drafts, tokens past the end: whole warp
@@ -289,52 +270,44 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
                 const bool past = p >= last || bad;
                 if (past) rvs[r] = 0.f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint32_t row = row0 + 8 * n + 2 * t + c;
-                        if (past || (p >= drafts && row < a.rows && !paged_sees(a, b, a.by_group.div(row), p - drafts)))
-                            s[n][2 * r + c] = -INFINITY;
-                    }
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t row = row0 + 2 * t + c;
+                    if (past || (p >= drafts && row < a.rows && !paged_sees(a, b, a.by_group.div(row), p - drafts)))
+                        s[2 * r + c] = -INFINITY;
+                }
             }
         }
 
         bool grow = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) grow |= fmaxf(s[n][c], s[n][2 + c]) > m[n][c] + kRefSlack;
+        for (int c = 0; c < 2; ++c) grow |= fmaxf(s[c], s[2 + c]) > m[c] + kRefSlack;
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int c = 0; c < 2; ++c) {
+                float mx = fmaxf(s[c], s[2 + c]);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float mx = fmaxf(s[n][c], s[n][2 + c]);
+                for (int off = 4; off <= 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                const float mn = fmaxf(m[c], mx - kRefBelow);
+                const float f = exp2f(m[c] - mn);
+                m[c] = mn;
+                l[c] *= f;
 #pragma unroll
-                    for (int off = 4; off <= 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                    const float mn = fmaxf(m[n][c], mx - kRefBelow);
-                    const float f = exp2f(m[n][c] - mn);
-                    m[n][c] = mn;
-                    l[n][c] *= f;
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        o[i][n][c] *= f;
-                        o[i][n][2 + c] *= f;
-                    }
+                for (int i = 0; i < MT; ++i) {
+                    o[i][c] *= f;
+                    o[i][2 + c] *= f;
                 }
+            }
         }
 
-        uint32_t p[NT][2];
+        uint32_t p[2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float w0 = ex2(s[n][2 * r] - m[n][0]), w1 = ex2(s[n][2 * r + 1] - m[n][1]);
-                l[n][0] = fmaf(w0, rvs[r], l[n][0]);
-                l[n][1] = fmaf(w1, rvs[r], l[n][1]);
-                const __half2 hw = __floats2half2_rn(w0, w1);
-                p[n][r] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&hw));
-            }
+        for (int r = 0; r < 2; ++r) {
+            const float w0 = ex2(s[2 * r] - m[0]), w1 = ex2(s[2 * r + 1] - m[1]);
+            l[0] = fmaf(w0, rvs[r], l[0]);
+            l[1] = fmaf(w1, rvs[r], l[1]);
+            const __half2 hw = __floats2half2_rn(w0, w1);
+            p[r] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&hw));
+        }
 
         TokenPair v[VW][2];
 #pragma unroll
@@ -342,45 +315,43 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
 #pragma unroll
             for (int half = 0; half < 2; ++half) v[j][half] = pair_tokens(x.v[2 * half][j], x.v[2 * half + 1][j]);
         if (more) load_v<D>(next, g, t, x);
-        pv_step<D, NT, 0>(v, p, o);
-        pv_step<D, NT, 1>(v, p, o);
-        pv_step<D, NT, 2>(v, p, o);
-        pv_step<D, NT, 3>(v, p, o);
+        pv_step<D, 0>(v, p, o);
+        pv_step<D, 1>(v, p, o);
+        pv_step<D, 2>(v, p, o);
+        pv_step<D, 3>(v, p, o);
     }
 
     // the warps' statistics and outputs, merged in warp order
     constexpr int rs = D + 4;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int off = 4; off <= 16; off <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], off);
+        float *dst = sm + (warp * kTileRows + 2 * t + c) * rs;
 #pragma unroll
-            for (int off = 4; off <= 16; off <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
-            float *dst = sm + (warp * ROWS + 8 * n + 2 * t + c) * rs;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if constexpr (D == 128) {  // tile i: channel 7 - i of blocks 2g and 2g + 1
-                    dst[16 * g + 7 - i] = o[i][n][c];
-                    dst[16 * g + 15 - i] = o[i][n][2 + c];
-                } else {  // tile i: channels 7 - i and 3 - i of block g
-                    dst[8 * g + 7 - i] = o[i][n][c];
-                    dst[8 * g + 3 - i] = o[i][n][2 + c];
-                }
-            }
-            if (g == 0) {
-                dst[D] = m[n][c];
-                dst[D + 1] = l[n][c];
+        for (int i = 0; i < MT; ++i) {
+            if constexpr (D == 128) {  // tile i: channel 7 - i of blocks 2g and 2g + 1
+                dst[16 * g + 7 - i] = o[i][c];
+                dst[16 * g + 15 - i] = o[i][2 + c];
+            } else {  // tile i: channels 7 - i and 3 - i of block g
+                dst[8 * g + 7 - i] = o[i][c];
+                dst[8 * g + 3 - i] = o[i][2 + c];
             }
         }
+        if (g == 0) {
+            dst[D] = m[c];
+            dst[D + 1] = l[c];
+        }
+    }
     // rows in turn to the warps of the CTA, or of the cluster, whose CTAs are then the splits
     const uint32_t ranks = a.clustered ? a.splits : 1, rank = a.clustered ? blockIdx.x : 0;
     if (a.clustered) cluster_sync();
     else __syncthreads();
-    for (uint32_t r = rank + ranks * warp; r < min((uint32_t)ROWS, a.rows - row0); r += ranks * kWarps) {
+    for (uint32_t r = rank + ranks * warp; r < min((uint32_t)kTileRows, a.rows - row0); r += ranks * kWarps) {
         float mx = kNoRef, ld = 0.f, od[D / 32] = {};
         for (uint32_t p = lane; p < ranks * kWarps; p += 32) {
             float st[2];
-            load_cluster(in_cta(sm + ((p % kWarps) * ROWS + r) * rs + D, p / kWarps), st);
+            load_cluster(in_cta(sm + ((p % kWarps) * kTileRows + r) * rs + D, p / kWarps), st);
             mx = fmaxf(mx, st[0]);
         }
 #pragma unroll
@@ -390,8 +361,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) paged_attn_kerne
             float st[kWarps][2], v[kWarps][D / 32];
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                load_cluster(base + (w * ROWS * rs + D) * 4, st[w]);
-                load_cluster(base + (w * ROWS * rs + lane * (D / 32)) * 4, v[w]);
+                load_cluster(base + (w * kTileRows * rs + D) * 4, st[w]);
+                load_cluster(base + (w * kTileRows * rs + lane * (D / 32)) * 4, v[w]);
             }
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
@@ -450,10 +421,10 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
 template <bool BF16, int D>
 int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st) {
     int status;
-    if (tile == 8) {
-        const dim3 grid(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, 8), batch);
-        status = launch_clustered(paged_attn_kernel<BF16, D, 1>, grid, a.clustered ? a.splits : 1, 32 * kWarps,
-                                  kWarps * 8 * (D + 4) * 4, st, a);
+    if (tile == kTileRows) {
+        const dim3 grid(a.splits, a.n_heads * (uint32_t)ceil_div(a.rows, kTileRows), batch);
+        status = launch_clustered(paged_attn_kernel<BF16, D>, grid, a.clustered ? a.splits : 1, 32 * kWarps,
+                                  kWarps * kTileRows * (D + 4) * 4, st, a);
     } else {
         status = launch_paged_tc(a, BF16, D, tile, batch, st);
     }
@@ -462,11 +433,20 @@ int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st
     return launch_overlapped(paged_combine_kernel<BF16, D>, dim3((unsigned)ceil_div(n, 4)), 128, 0, st, a, n);
 }
 
-// Rows of a CTA and tokens of a split.  The CTAs of a call come in rounds of
-// as many as the GPU holds, so the number of splits is the one whose rounds
-// times a CTA's time (its tiles, and kStartTiles tiles' worth of start and end)
-// is smallest, among those that fill two rounds where the tokens allow chunks
-// of kShortest tiles, for lengths that differ from the bound.  (Tree of 13 over
+// The kernel, its rows a CTA and the tokens of a split.
+//
+// Few rows go to the kernel of this file, the others to tcgen05.  A row tile
+// takes the decode again, so 16 rows of 128 channels are slower here (us, this
+// kernel : tcgen05; 8 KV heads): 377 : 278 for 32 x 16,384 tokens and 25 : 22 for 8 x
+// 2,048, where 8 rows are 197 : 247 for the first.  64 channels give a tile half the
+// decode: 16 rows 243 : 243 (32 x 16,384), 38.8 : 46.0 (8 x 8,192) and 9.5 : 12.0
+// (4 x 2,048), but 24 rows 341 : 269, 50.4 : 51.7 and 15.4 : 14.3.
+//
+// The CTAs of a call come in rounds of as many as the GPU holds, so the number
+// of splits is the one whose rounds times a CTA's time (its tiles, and
+// kStartTiles tiles' worth of start and end) is smallest, among those that fill
+// two rounds where the tokens allow chunks of kShortest tiles, for lengths that
+// differ from the bound.  (Tree of 13 over
 // 16 sequences of up to 8,190 tokens, mean over eight draws of their lengths:
 // no such floor 95.8 us, one round 81.2, two 80.7, three 81.3, five 93.9; tree
 // of 64 over 4 x 32,768 tokens: 5 splits 308 us, 6 326, 4 371.)
@@ -482,10 +462,11 @@ struct Plan {
 constexpr int64_t kClusterMax = 8, kClusterTokens = 256;  // splits, and the chunk up to which 8 of them are enough
 constexpr int64_t kStartTiles = 3, kShortest = 4, kMostSplits = 512;
 
-Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
+Plan plan(int64_t batch, int n_heads, int64_t rows, int head_dim, int64_t max_len) {
     Plan p;
-    p.tile = rows <= kFewRows ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    const int64_t tile_tokens = p.tile == 8 ? 64 : 128, slots = 148 * (p.tile == 8 ? 4 : 1);
+    const bool few = rows <= (head_dim == 64 ? 16 : 8);
+    p.tile = few ? kTileRows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    const int64_t tile_tokens = few ? 64 : 128, slots = 148 * (few ? 4 : 1);
     const int64_t units = batch * n_heads * ceil_div(rows, p.tile);  // CTAs without a split
     const int64_t tokens = max_len < 1 ? 1 : max_len, tiles = ceil_div(tokens, tile_tokens);
     int64_t best = 0, best_cost = INT64_MAX;
@@ -503,7 +484,7 @@ Plan plan(int64_t batch, int n_heads, int64_t rows, int64_t max_len) {
     if (best == 0) best = ceil_div(tiles, kMostSplits);
     p.chunk = best * tile_tokens;
     p.splits = (uint32_t)ceil_div(tokens, p.chunk);
-    p.clustered = p.tile == 8 && p.splits > 1 && (p.splits <= kClusterMax || tokens <= kClusterMax * kClusterTokens);
+    p.clustered = few && p.splits > 1 && (p.splits <= kClusterMax || tokens <= kClusterMax * kClusterTokens);
     if (p.clustered) {  // 2, 4 or 8 CTAs (the last may find nothing to do)
         p.splits = p.splits <= 2 ? 2 : p.splits <= 4 ? 4 : 8;
         p.chunk = ceil_div(ceil_div(tokens, p.splits), tile_tokens) * tile_tokens;
@@ -529,7 +510,7 @@ static bool paged_shape_ok(int64_t batch, int n_heads, int group, int64_t n_quer
 extern "C" size_t lq_paged_attention_workspace(int64_t batch, int n_heads, int group, int64_t n_query, int head_dim,
                                                int64_t max_len) {
     if (!paged_shape_ok(batch, n_heads, group, n_query, head_dim) || max_len < 0) return 0;
-    return workspace_of(plan(batch, n_heads, n_query * group, max_len), batch * n_heads * n_query * group, head_dim);
+    return workspace_of(plan(batch, n_heads, n_query * group, head_dim, max_len), batch * n_heads * n_query * group, head_dim);
 }
 
 extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
@@ -551,7 +532,7 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
     // tokens past max_len would have no split: the caller's bound is the table's at most
     const int64_t cap = table_width * page_tokens;
     const int64_t bound = max_len < cap ? max_len : cap;
-    const Plan p = plan(batch, n_heads, n_query * group, bound);
+    const Plan p = plan(batch, n_heads, n_query * group, head_dim, bound);
     if (const size_t need = workspace_of(p, batch * n_heads * n_query * group, head_dim)) {
         if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return LQ_ERR_INVALID;
         if (workspace_bytes < need) return LQ_ERR_CAPACITY;

@@ -117,7 +117,7 @@ __device__ __forceinline__ uint32_t bf16_to_f16(uint32_t x, float f) {
 }
 
 // The tensor-core kernel for many rows (lq_paged_attn_tc.cu): `tile` rows a
-// CTA, 8, 16, 32 or 64; a.chunk a multiple of 128.
+// CTA, 16, 32 or 64; a.chunk a multiple of 128.
 int launch_paged_tc(const PagedAttnArgs &a, bool bf16, int head_dim, int tile, uint32_t batch, cudaStream_t st);
 
 }  // namespace lq

@@ -7,7 +7,7 @@
 //   x = S^T * ks * c + log2(vs),  w = 2^(x - M),  l += w / vs
 //   O^T [D x N] += V^T [D x 128] W [128 x N]    (tcgen05.mma, stays in TMEM)
 // Tokens are the MMA's 128 rows, so no row is padding however few queries
-// there are; a thread owns one token (a TMEM lane) and half of the N columns.
+// there are; a softmax thread owns one token (a TMEM lane) and 16 of the N columns.
 //
 // The warps have four parts, which meet only at mbarriers:
 //   the producer  bulk-copies a tile's code words and scales, page by page, into
@@ -17,15 +17,17 @@
 //       read from the same token-major layout as an MN-major operand)
 //   two issuers start the two MMAs of every tile
 //   softmax    scores out of TMEM, weights to shared memory, a row of N per token
-// What a tile waits for in the last part, and with few rows in decoding, is
-// latency: 16 columns a thread keep enough warps there, with up to 32 rows two
-// sets of softmax warps take the tiles in turn, each with references,
-// denominators and an O of its own that are joined at the end, and with up to
-// 16 two sets of decoders do.
-// so copying, decoding, the tensor cores and the exponentials overlap.  64
-// positions over 4 sequences of 32,768 tokens (448 rows of 4 KV heads of 128):
-// 308 us, 390 TFLOP/s; mma.sync from registers took 749, and this kernel with
-// one barrier-synchronised part for all warps 413.
+// so copying, decoding, the tensor cores and the exponentials overlap.  What a
+// tile waits for in the last part, and with few rows in decoding, is latency: 16
+// columns a thread keep enough warps there, with up to 32 rows two sets of
+// softmax warps take the tiles in turn, each with references, denominators and
+// an O of its own that are joined at the end, and with up to 16 two sets of
+// decoders do.
+//
+// 64 positions over 4 sequences of 32,768 tokens (448 rows of 4 KV heads of 128):
+// 308 us, 390 TFLOP/s, bound by issue: 7,290 instructions and 2,940 cycles a tile
+// of 128 tokens and 64 rows.  Earlier forms of the product took 749 us (mma.sync
+// from registers) and 413 (tcgen05 with one barrier-synchronised part).
 //
 // M is a reference per row, moved only when an x exceeds it by kRefSlack,
 // which a vote of the 128 threads finds; O is then rescaled in TMEM.
@@ -192,8 +194,8 @@ __device__ __forceinline__ float fold(float (&v)[C], Op op) {
 // The kernel for D channels and up to COLS query rows a CTA.
 template <int D, int COLS>
 struct Shape {
-    static constexpr int kN = COLS < 16 ? 16 : COLS;   // columns of the MMAs
-    static constexpr int kC = COLS < 16 ? COLS : 16;   // columns of a softmax thread
+    static constexpr int kN = COLS;                    // columns of the MMAs
+    static constexpr int kC = 16;                      // columns of a softmax thread
     static constexpr int kGroups = COLS / kC;          // column groups of 4 warps
     static constexpr int kSets = COLS <= 32 ? 2 : 1;   // of softmax warps, which take the tiles in turn
     static constexpr int kSoftmax = 4 * kGroups * kSets;
@@ -639,8 +641,9 @@ int launch_n(const PagedAttnArgs &a, uint32_t batch, cudaStream_t st) {
 
 template <bool BF16, int D>
 int launch_d(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st) {
-    if (tile == 8) return launch_n<BF16, D, 8>(a, batch, st);
-    if (tile == 16) return launch_n<BF16, D, 16>(a, batch, st);
+    if constexpr (D == 128) {  // up to 16 rows of 64 channels go to the other kernel
+        if (tile == 16) return launch_n<BF16, D, 16>(a, batch, st);
+    }
     if (tile == 32) return launch_n<BF16, D, 32>(a, batch, st);
     return launch_n<BF16, D, 64>(a, batch, st);
 }

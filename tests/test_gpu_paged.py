@@ -590,3 +590,30 @@ def test_append_equals_the_frameworks_search_at_its_ties(P, dtype):
         assert torch.equal(k, (q * s[..., None]).to(dtype))
         stored = _values(codes[0, :, 0], scales[0, :, 0]).transpose(0, 2, 1, 3).reshape(n, H, D)
         assert np.array_equal(stored, q.double().cpu().numpy() * s[..., None].double().cpu().numpy())
+
+
+@pytest.mark.parametrize("lens,H,G,T,dtype,mask", [
+    ([9, 10, 200, 64], 2, 3, 3, torch.bfloat16, "batch"),     # 9 rows: one in the last tile
+    ([1, 2030, 0], 1, 4, 4, torch.float16, "one"),            # 16, fewer tokens than positions
+    ([5000, 11], 3, 1, 11, torch.bfloat16, "causal"),
+    ([16385], 1, 15, 1, torch.float16, None),
+])
+def test_attention_two_row_tiles(P, lens, H, G, T, dtype, mask):
+    """9 to 16 rows of 64 channels, with rows that see nothing and entries outside the pool."""
+    from latticequant_b200 import _lib
+
+    g = torch.Generator(device="cuda").manual_seed(T)
+    codes, scales, table, ln = _pool(P, g, lens, H, 64, 16, spread=1.0)
+    q = torch.randn(len(lens), H * G, T, 64, device="cuda", generator=g).to(dtype)
+    m = None if mask in (None, "causal") else _tree(T, T, len(lens) if mask == "batch" else None)
+    if m is not None:
+        m[..., 1, :] = False
+    o, lse = P.tree_attention(q, codes, scales, table, ln, m, return_lse=True)
+    _check(o, lse, *_ref(q, codes, scales, table, lens, m, 1 / 8))
+    assert torch.equal(o, P.tree_attention(q, codes, scales, table, ln, m))
+    for entry in (-1, codes.shape[0], 2**31 - 1):
+        bad = table.clone()
+        bad[0, 0] = entry
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        o = P.tree_attention(q, codes, scales, bad, ln, m, err=err)
+        assert int(err.item()) == _lib.EF_PAGE and torch.isfinite(o).all()
