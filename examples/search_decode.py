@@ -6,9 +6,11 @@ A small randomly initialised decoder (no weights are needed) runs the three
 loops that a server runs over ``llm.paged_cache.PagedKVCache``:
 
 * greedy decoding, one token a step;
-* the same tokens from trees of drafts: each step checks a tree and keeps the
+* greedy decoding from trees of drafts: each step checks a tree and keeps the
   longest path the model confirms (half of the drafts here are right, so the
-  loop takes fewer steps);
+  loop takes fewer steps).  A tree's sums run in another order than a single
+  token's, so where two logits of this bfloat16 model are closer than its
+  rounding, either may win and the two loops part;
 * beam search: beam_select picks the continuations, fork reorders the cache.
 
 Prints the steps each took and whether the tree's tokens are the greedy ones.
