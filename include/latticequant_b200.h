@@ -479,7 +479,8 @@ int lq_paged_append(const void *k, const void *v, int dtype, int64_t n_tokens, i
  *            (longer ones are cut, with LQ_EF_PAGE)
  *   mask     bytes [n_query][n_query], sequences mask_stride_b apart (0: one
  *            for all); NULL: causal
- *   out      [batch][n_heads * group][n_query][head_dim] in q's type
+ *   out      [batch][n_heads * group][n_query][head_dim] in q's type, aligned
+ *            to head_dim / 16 bytes
  *   lse      optional fp32 [batch][n_heads * group][n_query], natural log.  A
  *            position that sees no token gets o = 0, lse = -inf
  * n_query 1..4096, group 1..64. */

@@ -529,6 +529,8 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
     const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(codes) |
                          reinterpret_cast<uintptr_t>(scales);
     if ((al & 15) != 0 || ((q_stride_b | q_stride_h | q_stride_t) & 7) != 0) return LQ_ERR_INVALID;
+    // a lane stores head_dim / 32 elements at once
+    if ((reinterpret_cast<uintptr_t>(out) & (head_dim / 16 - 1)) != 0) return LQ_ERR_INVALID;
     // tokens past max_len would have no split: the caller's bound is the table's at most
     const int64_t cap = table_width * page_tokens;
     const int64_t bound = max_len < cap ? max_len : cap;

@@ -142,7 +142,8 @@ def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, t
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _need(out, dtype, (B, Hq, T, D), "out", index)
+        if _need(out, dtype, (B, Hq, T, D), "out", index) % (D // 16):
+            raise ValueError(f"out must be aligned to {D // 16} bytes")
     lse = lens.new_empty((B, Hq, T), dtype=_F32) if return_lse else None
     bound = width * P if max_len is None else min(int(max_len), width * P)
     need = _attention_workspace(B, H, Hq // H, T, D, bound)

@@ -1,0 +1,37 @@
+"""The paged cache at its limits: what it refuses, reports and survives."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def P():
+    from latticequant_b200 import paged
+
+    return paged
+
+
+def _filled(P, lens, H, D, page, seed=0, dtype=torch.float16):
+    """(codes, scales, table, lens) of one layer: sequence b holds lens[b] random tokens in pages of its own."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    width = max(1, -(-max(lens) // page))
+    codes, scales, _ = P.empty_pool(1, len(lens) * width, H, D, page)
+    table = torch.arange(len(lens) * width, device="cuda", dtype=torch.int32).view(-1, width)
+    for b, n in enumerate(lens):
+        pos = torch.arange(n, device="cuda")
+        kv = torch.randn(2, n, H, D, device="cuda", generator=g).to(dtype)
+        P.append(codes[0], scales[0], kv[0], kv[1], table[b, pos // page].long() * page + pos % page)
+    return codes[0], scales[0], table, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("D,off", [(64, 1), (128, 1), (128, 2)])
+def test_misaligned_outputs_are_refused(P, D, off):
+    codes, scales, table, ln = _filled(P, [40], 2, D, 16)
+    q = torch.randn(1, 4, 1, D, device="cuda").to(torch.float16)
+    buf = torch.zeros(4 * D + 8, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="aligned"):
+        P.tree_attention(q, codes, scales, table, ln, out=buf[off: off + 4 * D].view(1, 4, 1, D))
+    fine = D // 32  # the least that the stores take
+    o = P.tree_attention(q, codes, scales, table, ln, out=buf[fine: fine + 4 * D].view(1, 4, 1, D))
+    assert torch.equal(o, P.tree_attention(q, codes, scales, table, ln))

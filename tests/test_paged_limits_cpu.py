@@ -1,0 +1,20 @@
+"""What the paged cache's C entry points have to refuse, or to size, before anything is launched (no GPU)."""
+import pytest
+
+INVALID, CAPACITY = -1, -3
+PTR = 4096  # aligned and never dereferenced: every call below is refused
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from latticequant_b200 import _lib
+
+    return _lib.lib()
+
+
+@pytest.mark.parametrize("dim,bytes_", [(64, 4), (128, 8)])
+def test_attention_refuses_outputs_that_its_stores_cannot_take(lib, dim, bytes_):
+    """A lane stores head_dim / 32 elements of 16 bits at once."""
+    for off in range(1, bytes_):
+        assert lib.lq_paged_attention(PTR, 1, dim, dim, dim, PTR, PTR, 4, 16, PTR, 4, 4, PTR, 64, None, 0, 1, 1, 1, 1, dim,
+                                      1.0, PTR + off, None, None, 0, None, None) == INVALID
