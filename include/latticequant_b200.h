@@ -517,7 +517,7 @@ int lq_pages_compact(const int32_t *table, int64_t entries, const int32_t *refs,
                      int64_t n_pages, int n_heads, int page_tokens, int head_dim, void *workspace,
                      size_t workspace_bytes, uint32_t *err, void *stream);
 
-/* Copy pages src[i] to dst[i], i < *count (on the device, at most `most`), in
+/* Copy pages src[i] to dst[i], i < min(*count, most) (count on the device), in
  * all layers; no dst is a src and no dst is named twice. */
 int lq_pages_copy(const int32_t *src, const int32_t *dst, const int32_t *count, int64_t most, int32_t *codes,
                   float *scales, int64_t n_layers, int64_t n_pages, int n_heads, int page_tokens, int head_dim,

@@ -198,7 +198,8 @@ struct MoveArgs {
     const int32_t *table;
     int64_t entries, n_pages;
     int32_t *new_table, *new_refs, *n_live;
-    int32_t *src, *dst, *count;  // the moves; `to`: a page's new place
+    int32_t *src, *dst, *count;  // the moves, at most `most`; `to`: a page's new place
+    int64_t most;
     int32_t *to;
     uint32_t *codes;
     float *scales;
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(256) move_pages_kernel(const __grid_constant__
             a.new_table[e] = p >= 0 && p < a.n_pages ? a.to[p] : -1;
             if (p >= a.n_pages) raise_flag(a.err, LQ_EF_PAGE);
         }
-    const int64_t units = (int64_t)*a.count * a.n_layers;
+    const int64_t units = min((int64_t)*a.count, a.most) * a.n_layers;
     const int64_t cv = a.page_rows * a.W / 4, sv = a.page_rows / 4;  // 16-byte vectors (P is a multiple of 16)
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const int64_t i = u / a.n_layers, layer = (u - i * a.n_layers) * a.n_pages;
@@ -436,6 +437,7 @@ extern "C" int lq_pages_compact(const int32_t *table, int64_t entries, const int
     a.new_refs = new_refs;
     a.n_live = n_live;
     a.count = static_cast<int32_t *>(workspace);
+    a.most = n_pages;
     a.src = a.count + 1;
     a.dst = a.src + n_pages;
     a.to = a.dst + n_pages;
@@ -464,6 +466,7 @@ extern "C" int lq_pages_copy(const int32_t *src, const int32_t *dst, const int32
     a.src = const_cast<int32_t *>(src);
     a.dst = const_cast<int32_t *>(dst);
     a.count = const_cast<int32_t *>(count);
+    a.most = most;
     a.codes = reinterpret_cast<uint32_t *>(codes);
     a.scales = scales;
     a.n_layers = n_layers;

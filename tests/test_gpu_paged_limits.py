@@ -35,3 +35,17 @@ def test_misaligned_outputs_are_refused(P, D, off):
     fine = D // 32  # the least that the stores take
     o = P.tree_attention(q, codes, scales, table, ln, out=buf[fine: fine + 4 * D].view(1, 4, 1, D))
     assert torch.equal(o, P.tree_attention(q, codes, scales, table, ln))
+
+
+def test_copy_reads_no_pair_past_the_lists(P):
+    """A count above the lists' length copies the listed pairs and no other."""
+    codes = torch.randint(-2**31, 2**31 - 1, (2, 9, 2, 1, 16, 8), dtype=torch.int32, device="cuda")
+    scales = torch.rand(2, 9, 2, 1, 16, device="cuda")
+    c0, s0 = codes.clone(), scales.clone()
+    src, dst = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([3, 0, 5, 6], [8, 2, 1, 7]))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for count in (7, 2**31 - 1, 0, -1):  # the lists end before their memory does
+        P.copy_pages(codes, scales, src[:2], dst[:2], torch.tensor([count], dtype=torch.int32, device="cuda"), err)
+        if count > 0:
+            c0[:, [8, 2]], s0[:, [8, 2]] = c0[:, [3, 0]], s0[:, [3, 0]]
+        assert torch.equal(codes, c0) and torch.equal(scales, s0) and int(err.item()) == 0
