@@ -383,6 +383,7 @@ extern "C" int lq_pages_fork(const int32_t *table, int64_t rows, int64_t width, 
     if (!refs || !new_refs || (rows > 0 && (!table || !lens)) || (children > 0 && (!parents || !new_table || !new_lens)) ||
         !workspace)
         return LQ_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 3) != 0) return LQ_ERR_INVALID;
     if (workspace_bytes < lq_pages_fork_workspace(rows, children, n_pages)) return LQ_ERR_CAPACITY;
     ForkArgs a{};
     a.table = table;
@@ -427,6 +428,7 @@ extern "C" int lq_pages_compact(const int32_t *table, int64_t entries, const int
     LQ_NVTX_RANGE();
     if (!pool_ok(codes, scales, n_layers, n_pages, n_heads, page_tokens, head_dim) || entries < 0) return LQ_ERR_INVALID;
     if (!refs || !new_refs || !n_live || (entries > 0 && (!table || !new_table)) || !workspace) return LQ_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 3) != 0) return LQ_ERR_INVALID;
     if (workspace_bytes < lq_pages_compact_workspace(n_pages)) return LQ_ERR_CAPACITY;
     MoveArgs a{};
     a.refs = refs;

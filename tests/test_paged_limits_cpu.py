@@ -18,3 +18,12 @@ def test_attention_refuses_outputs_that_its_stores_cannot_take(lib, dim, bytes_)
     for off in range(1, bytes_):
         assert lib.lq_paged_attention(PTR, 1, dim, dim, dim, PTR, PTR, 4, 16, PTR, 4, 4, PTR, 64, None, 0, 1, 1, 1, 1, dim,
                                       1.0, PTR + off, None, None, 0, None, None) == INVALID
+
+
+def test_page_operations_refuse_misaligned_workspaces(lib):
+    """The workspaces hold 32-bit words."""
+    for off in (1, 2, 3):
+        assert lib.lq_pages_fork(PTR, 2, 4, PTR, PTR, PTR, 2, 0, PTR, PTR, PTR, PTR, PTR, 1, 8, 1, 16, 64, PTR + off, 1 << 20,
+                                 None, None) == INVALID
+        assert lib.lq_pages_compact(PTR, 8, PTR, PTR, PTR, PTR, PTR, PTR, 1, 8, 1, 16, 64, PTR + off, 1 << 20, None,
+                                    None) == INVALID
