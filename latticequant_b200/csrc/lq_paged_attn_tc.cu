@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
     __syncthreads();
     tmem_fence_after();
     const uint32_t ts = sm.tmem, to = ts + 2 * N;
-    Waiter wait;
+    Waiter wait, drain;
 
     if (warp < X::kSoftmax) {
         // ---- softmax: token tl (a TMEM lane), columns col0.., every kSets-th tile
@@ -550,14 +550,17 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
         // ---- the issuers (the first warp starts S, the second O) and the producer
         const int issuer = __shfl_sync(0xffffffffu, warp - X::kIssue, 0);  // uniform
         const uint32_t one = elect_lane();
+        // Nothing of this block's is under way when it ends: what an issuer or the producer has started arrives
+        // first, also where a wait gave up (it starts nothing more then).
         if (issuer == 0) {
             const uint64_t dq = operand(sq, 16, 1024), dk = operand(sk, 16, 1024);
             wait(sm.q_full, 0);
-            for (int j = 0; j < n_tiles; ++j) {
+            int j = 0;
+            for (; j < n_tiles; ++j) {
                 const int s = j & 1;
                 wait(sm.k_full[s], j >> 1);
                 if (j >= 2) wait(sm.s_free[s], (j >> 1) - 1);
-                __syncwarp();
+                if (__any_sync(0xffffffffu, !wait.alive)) break;
                 tmem_fence_after();
                 const uint64_t dks = dk + (uint32_t)(s * (X::kTileBytes >> 4));
                 mma<false>(ts + s * N, dks, dq, kShape<N>, one);
@@ -570,14 +573,16 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
                 mma_done(smem_u32(&sm.s_full[s]), one);
                 mma_done(smem_u32(&sm.k_free[s]), one);
             }
+            for (int i = max(j - 2, 0); i < j; ++i) drain(sm.k_free[i & 1], i >> 1);
         } else if (issuer == 1) {
             constexpr uint32_t shape = kShape<N> | kTransposeA | kTransposeB;
             const uint64_t dp = operand(sp, kHalfBytes, 1024), dv = operand(sv, kHalfBytes, 1024);
-            for (int j = 0; j < n_tiles; ++j) {
+            int j = 0;
+            for (; j < n_tiles; ++j) {
                 const int s = j & 1, set = j % X::kSets, turn = j / X::kSets;
                 wait(sm.v_full[s], j >> 1);
                 wait(sm.p_full[set], turn);
-                __syncwarp();
+                if (__any_sync(0xffffffffu, !wait.alive)) break;
                 tmem_fence_after();
                 const uint64_t dvs = dv + (uint32_t)(s * (X::kTileBytes >> 4)), dps = dp + set * (kHalfBytes >> 4);
                 const uint32_t d = to + set * N;
@@ -588,18 +593,20 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
                 mma_done(smem_u32(&sm.p_free[set]), one);
                 mma_done(smem_u32(&sm.v_free[s]), one);
             }
+            for (int i = max(j - 2, 0); i < j; ++i) drain(sm.v_free[i & 1], i >> 1);
         } else if (issuer == 2) {
             // lane i < segs copies the tile's i-th run of rows that lie in one page
             const int64_t side = (int64_t)a.n_heads << a.page_log2;
             const uint32_t *kbase = a.codes + ((int64_t)h << a.page_log2) * W;
             const float *sbase = a.scales + ((int64_t)h << a.page_log2);
-            int stage = 0;
-            for (int j = 0; j < n_tiles; ++j, tok_p += kTok) {
+            int stage = 0, j = 0;
+            for (; j < n_tiles; ++j, tok_p += kTok) {
                 const int tok = tok_p;
                 const bool mine = lane < segs && tok < last, bad = mine && (uint32_t)page >= (uint32_t)a.n_pages;
                 const int64_t row = 2 * side * (bad ? 0 : page) + (tok & ((1 << a.page_log2) - 1));
                 page = entry_of(tok + kTok);
                 if (j >= X::kStages) wait(sm.stage_free[stage], j / X::kStages - 1);
+                if (__any_sync(0xffffffffu, !wait.alive)) break;
                 const uint32_t runs = __popc(__ballot_sync(0xffffffffu, mine)), out = __ballot_sync(0xffffffffu, bad);
                 const uint32_t bar = smem_u32(&sm.stage_full[stage]);
                 if (lane == 0) {
@@ -618,9 +625,10 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
                 }
                 stage = stage == X::kStages - 1 ? 0 : stage + 1;
             }
+            for (int i = max(j - X::kStages, 0); i < j; ++i) drain(sm.stage_full[i % X::kStages], i / X::kStages);
         }
     }
-    if (!wait.alive) raise_flag(a.err, LQ_EF_TIMEOUT);
+    if (!wait.alive || !drain.alive) raise_flag(a.err, LQ_EF_TIMEOUT);
     __syncthreads();
     if (warp == X::kIssue)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(ts), "r"(X::kTmem) : "memory");

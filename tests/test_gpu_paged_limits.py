@@ -49,3 +49,20 @@ def test_copy_reads_no_pair_past_the_lists(P):
         if count > 0:
             c0[:, [8, 2]], s0[:, [8, 2]] = c0[:, [3, 0]], s0[:, [3, 0]]
         assert torch.equal(codes, c0) and torch.equal(scales, s0) and int(err.item()) == 0
+
+
+@pytest.mark.parametrize("G,T,D", [(4, 4, 128), (4, 8, 128), (8, 8, 128), (3, 10, 64), (8, 8, 64)])
+def test_short_blocks_leave_nothing_behind(P, G, T, D):
+    """One or two tiles a block and many blocks a SM in a row: a block's last arrivals come before it ends, so its
+    successor in the same shared memory answers as it does alone."""
+    lens = [T + (37 * b) % 230 for b in range(96)]
+    codes, scales, table, ln = _filled(P, lens, 4, D, 64)
+    q = torch.randn(len(lens), 4 * G, T, D, device="cuda").to(torch.float16)
+    alone = torch.cat([P.tree_attention(q[b: b + 1], codes, scales, table[b: b + 1], ln[b: b + 1], max_len=256)
+                       for b in range(len(lens))])
+    o = P.tree_attention(q, codes, scales, table, ln, max_len=256)
+    # (the split, and so the order of the sums, is that of the batch: fp16's unit roundoff and a weight's, twice)
+    top = alone.float().abs().amax(-1, keepdim=True)
+    assert bool(((o.float() - alone.float()).abs() <= 2e-3 * top + 2 ** -10 * alone.float().abs()).all())
+    for _ in range(20):
+        assert torch.equal(o, P.tree_attention(q, codes, scales, table, ln, max_len=256))
