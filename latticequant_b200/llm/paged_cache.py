@@ -56,9 +56,10 @@ class PagedKVCache:
         self.fork(torch.arange(self.rows, device=self.table.device), reserve=n)
         p = self.page_tokens
         at = self.lens.long()[:, None] + torch.arange(n, device=self.table.device)
-        page = self.table.gather(1, (at // p).clamp_(max=self.table.shape[1] - 1)).long()
-        # no page (too few free ones: flags() says so): not stored
-        self._slots = torch.where(page >= 0, page * p + at % p, -1).reshape(-1)
+        width = self.table.shape[1]
+        page = self.table.gather(1, (at // p).clamp_(max=width - 1)).long()
+        # not stored (flags() says so): tokens without a page, whose slot is negative, and those past the table
+        self._slots = torch.where(at < width * p, page * p + at % p, -1).reshape(-1)
         self.lens = self.lens + n
         self.max_len += n
         self._n_new = n

@@ -66,3 +66,58 @@ def test_short_blocks_leave_nothing_behind(P, G, T, D):
     assert bool(((o.float() - alone.float()).abs() <= 2e-3 * top + 2 ** -10 * alone.float().abs()).all())
     for _ in range(20):
         assert torch.equal(o, P.tree_attention(q, codes, scales, table, ln, max_len=256))
+
+
+def _cache(rows, n_pages=24, max_tokens=64, page=16, layers=1):
+    from latticequant_b200.llm.paged_cache import PagedKVCache
+
+    return PagedKVCache(layers, 2, 64, n_pages=n_pages, rows=rows, max_tokens=max_tokens, page_tokens=page)
+
+
+def _kv(g, rows, n):
+    return [torch.randn(rows, 2, n, 64, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2)]
+
+
+@pytest.mark.parametrize("n", [1, 20, 40])
+def test_tokens_past_the_table_are_not_stored(n):
+    """Rows that are as long as their table allows keep what they hold, and so do the rows that share their pages."""
+    from latticequant_b200 import _lib
+
+    g = torch.Generator(device="cuda").manual_seed(n)
+    c = _cache(2)
+    c.begin(64)
+    c.append(0, *_kv(g, 2, 64))
+    c.fork(torch.tensor([0, 0, 1], device="cuda"))
+    q = torch.randn(3, 4, 1, 64, device="cuda", generator=g).to(torch.bfloat16)
+    before, codes, scales = c.attend(0, q), c.codes.clone(), c.scales.clone()
+    assert c.flags() == 0
+    c.begin(n)
+    k, v = c.append(0, *_kv(g, 3, n), dequantised=True)
+    assert c.flags() & _lib.EF_PAGE and k.shape == (3, 2, n, 64)
+    assert torch.equal(c.codes, codes) and torch.equal(c.scales, scales)
+    c.lens = (c.lens - n).clamp_(max=64)
+    c.max_len = 64
+    assert torch.equal(c.attend(0, q), before)
+
+
+def test_tokens_up_to_the_tables_end_are_stored():
+    """A row one token short of its table stores that token and drops the next; a shorter row beside it stores both."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    c, one = _cache(2), _cache(1)
+    kv = _kv(g, 2, 63)
+    c.begin(63)
+    c.append(0, *kv)
+    c.fork(torch.tensor([0, 1], device="cuda"))
+    c.lens = torch.tensor([63, 30], dtype=torch.int32, device="cuda")
+    new = _kv(g, 2, 2)
+    c.begin(2)
+    c.append(0, *new)
+    one.begin(64)
+    one.append(0, *[torch.cat([x[:1], y[:1, :, :1]], 2) for x, y in zip(kv, new)])
+    page, row = int(c.table[0, 3]), int(one.table[0, 3])
+    assert torch.equal(c.codes[0, page], one.codes[0, row]) and torch.equal(c.scales[0, page], one.scales[0, row])
+    short = _cache(1)
+    short.begin(32)
+    short.append(0, *[torch.cat([x[1:, :, :30], y[1:]], 2) for x, y in zip(kv, new)])
+    for col in range(2):
+        assert torch.equal(c.codes[0, int(c.table[1, col])], short.codes[0, int(short.table[0, col])])
