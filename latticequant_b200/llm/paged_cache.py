@@ -54,15 +54,18 @@ class PagedKVCache:
     def begin(self, n: int) -> None:
         """Make room for n tokens a row and count them in."""
         self.fork(torch.arange(self.rows, device=self.table.device), reserve=n)
-        p = self.page_tokens
-        at = self.lens.long()[:, None] + torch.arange(n, device=self.table.device)
-        width = self.table.shape[1]
-        page = self.table.gather(1, (at // p).clamp_(max=width - 1)).long()
-        # not stored (flags() says so): tokens without a page, whose slot is negative, and those past the table
-        self._slots = torch.where(at < width * p, page * p + at % p, -1).reshape(-1)
         self.lens = self.lens + n
         self.max_len += n
         self._n_new = n
+        self._slots = self._slots_of_last(n)
+
+    def _slots_of_last(self, n: int) -> torch.Tensor:
+        """Where each row's last n tokens go, (rows * n,) int64."""
+        p, width = self.page_tokens, self.table.shape[1]
+        at = self.lens.long()[:, None] + torch.arange(-n, 0, device=self.table.device)
+        page = self.table.gather(1, (at // p).clamp_(max=width - 1)).long()
+        # not stored (flags() says so): tokens without a page, whose slot is negative, and those past the table
+        return torch.where(at < width * p, page * p + at % p, -1).reshape(-1)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, dequantised: bool = False
                ) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
@@ -103,6 +106,8 @@ class PagedKVCache:
     def compact(self) -> torch.Tensor:
         """Move the pages in use to the front of the pool; their number, (1,) int32 on the device."""
         self.table, self.refs, n_live = paged.compact_pages(self.codes, self.scales, self.table, self.refs, self.err)
+        if self._slots is not None:  # in a step: the rest of its tokens go where the pages are now
+            self._slots = self._slots_of_last(self._n_new)
         return n_live
 
     def flags(self) -> int:

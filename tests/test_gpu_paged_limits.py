@@ -121,3 +121,27 @@ def test_tokens_up_to_the_tables_end_are_stored():
     short.append(0, *[torch.cat([x[1:, :, :30], y[1:]], 2) for x, y in zip(kv, new)])
     for col in range(2):
         assert torch.equal(c.codes[0, int(c.table[1, col])], short.codes[0, int(short.table[0, col])])
+
+
+def test_compaction_within_a_step():
+    """Pages renamed between begin() and the last layer's append(): the rest of the step follows them."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ctx, new = _kv(g, 4, 30), _kv(g, 4, 5)
+    q = torch.randn(4, 4, 5, 64, device="cuda", generator=g).to(torch.bfloat16)
+    out = []
+    for compact in (False, True):
+        c = _cache(4, layers=2)
+        c.begin(30)
+        c.append(0, *ctx)
+        c.append(1, *ctx)
+        c.free(torch.tensor([0, 1, 2], device="cuda"))  # holes below the other row's pages
+        c.begin(5)
+        c.append(0, *new)
+        if compact:
+            n = c.compact()
+            assert int(c.table.max()) == int(n) - 1
+        c.append(1, *new)
+        out.append([c.attend(layer, q) for layer in range(2)] + [c.lens])
+        assert c.flags() == 0
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
