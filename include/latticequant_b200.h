@@ -496,8 +496,9 @@ int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q
 /* Fork, free and reserve: new tables whose row i continues row parents[i] of
  * the old ones (-1: an empty row; rows named by no child are freed), with
  * pages for `reserve` more tokens.  Full pages are shared.  The page a row
- * writes to next, and reserved ones, stay with the row's first child; other
- * children get fresh pages, the lowest free ones in order of child and
+ * writes to next, and reserved ones, stay with the row's first child where
+ * refs is 1; other children, and every child of a row whose page somebody else
+ * names too, get fresh pages, the lowest free ones in order of child and
  * column, with the live rows copied in all layers.  Entries past the reserve
  * are -1.  Out of place: outputs alias no input.  Too few free pages leave
  * -1 entries and raise LQ_EF_CAPACITY. */

@@ -86,9 +86,13 @@ __device__ __forceinline__ Child child_of(const ForkArgs &a, int64_t i) {
     return c;
 }
 
-// Whether child c keeps its parent's page of column col >= full.
+// Whether child c keeps its parent's page of column col >= full: it will write
+// there, so no other entry may name the page (rows that went back behind the
+// point of a fork share pages that they had filled).
 __device__ __forceinline__ bool keeps(const ForkArgs &a, const Child &c, int64_t col) {
-    return c.first && a.table[c.parent * a.width + col] >= 0;
+    if (!c.first) return false;
+    const int32_t p = a.table[c.parent * a.width + col];
+    return p >= 0 && (p >= a.n_pages || a.refs[p] <= 1);
 }
 
 // One CTA: owners, fresh pages of each child, the free list, a copy of the counts.
@@ -185,7 +189,7 @@ __global__ void __launch_bounds__(256) fork_apply_kernel(const __grid_constant__
     if (i >= a.children) return;
     const Child c = child_of(a, i);
     const int n = (int)(c.len & ((1 << a.page_log2) - 1));
-    if (c.parent < 0 || c.first || n == 0 || c.full >= c.need || a.base[i] >= a.fresh_cap) return;
+    if (c.parent < 0 || n == 0 || c.full >= c.need || a.base[i] >= a.fresh_cap || keeps(a, c, c.full)) return;
     const int32_t src = a.table[c.parent * a.width + c.full], dst = a.fresh[a.base[i]];
     if (src < 0 || src >= a.n_pages || dst < 0) return;
     const int64_t layer = (int64_t)(blockIdx.y - 1) * a.n_pages;

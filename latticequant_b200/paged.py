@@ -167,8 +167,8 @@ def fork_pages(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, l
     an empty row), with pages for ``reserve`` more tokens (lq_pages_fork).
 
     Full pages are shared; the page a row writes to next stays with the row's
-    first child, the others get a copy of its live rows in a fresh page.  Rows
-    that no child names are freed.  parents = arange reserves, parents with -1
+    first child if nobody else names it (refs 1), the others get a copy of its
+    live rows in a fresh page.  Rows that no child names are freed.  parents = arange reserves, parents with -1
     entries free rows, repeated parents fork: beam search's reordering is
     parents = the selected beams."""
     index, n_pages, H, P, D = _pool(codes, scales, 6)

@@ -145,3 +145,57 @@ def test_compaction_within_a_step():
         assert c.flags() == 0
     for a, b in zip(*out):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("reserve", [0, 3, 40])
+def test_fork_copies_a_shared_page_that_is_written_next(P, reserve):
+    """Rows 0 and 1 both name page 5, of which they hold 9 tokens: neither may write there."""
+    L, H, page, D = 2, 3, 16, 64
+    codes = torch.randint(-2**31, 2**31 - 1, (L, 20, 2, H, page, D // 8), dtype=torch.int32, device="cuda")
+    scales = torch.rand(L, 20, 2, H, page, device="cuda")
+    old = [[2, 5, 7, -1, -1], [2, 5, -1, -1, -1], [9, 1, 7, -1, -1]]  # a shared page past the first one to write, too
+    table = torch.tensor(old, dtype=torch.int32, device="cuda")
+    lens = [25, 25, 32]
+    refs = torch.bincount(table[table >= 0].long(), minlength=20).to(torch.int32)
+    c0, s0 = codes.clone(), scales.clone()
+    parents, err = [0, 1, 2, 0], torch.zeros(1, dtype=torch.int32, device="cuda")
+    t, n, r = P.fork_pages(codes, scales, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), refs,
+                           torch.tensor(parents, device="cuda"), reserve, err)
+    assert int(err.item()) == 0 and n.tolist() == [25, 25, 32, 25]
+    free, want = [i for i in range(20) if int(refs[i]) == 0], []
+    for p in parents:
+        full, need = lens[p] // page, -(-(lens[p] + reserve) // page)
+        row = old[p][:full] + [free.pop(0) for _ in range(full, need)]  # no page of theirs is their own
+        if lens[p] % page:
+            c0[:, row[full], :, :, : lens[p] % page] = c0[:, old[p][full], :, :, : lens[p] % page]
+            s0[:, row[full], :, :, : lens[p] % page] = s0[:, old[p][full], :, :, : lens[p] % page]
+        want.append(row + [-1] * (5 - len(row)))
+    assert t.tolist() == want
+    assert torch.equal(r, torch.bincount(t[t >= 0].long(), minlength=20).to(torch.int32))
+    assert torch.equal(codes, c0) and torch.equal(scales, s0)
+
+
+def test_rollback_behind_a_fork():
+    """Drafts are rejected after a fork shared the page that they filled: the rows go on apart, as rows of their own would."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    ctx, drafts = _kv(g, 1, 14), _kv(g, 1, 5)
+    c = _cache(1)
+    c.begin(14)
+    c.append(0, *ctx)
+    c.begin(5)
+    c.append(0, *drafts)
+    c.fork(torch.tensor([0, 0], device="cuda"))  # 19 tokens: page 0 is full, and shared
+    c.accept(torch.full((2, 1), -1, dtype=torch.int32, device="cuda"))
+    new = [_kv(g, 2, 1) for _ in range(4)]
+    for kv in new:
+        c.begin(1)
+        c.append(0, *kv)
+    assert c.lens.tolist() == [18, 18] and c.flags() == 0
+    q = torch.randn(2, 4, 1, 64, device="cuda", generator=g).to(torch.bfloat16)
+    o = c.attend(0, q)
+    for b in range(2):
+        own = _cache(1)
+        own.begin(18)
+        own.append(0, *[torch.cat([x] + [kv[i][b: b + 1] for kv in new], 2) for i, x in enumerate(ctx)])
+        assert torch.equal(o[b: b + 1], own.attend(0, q[b: b + 1]))
+    assert torch.equal(c.refs, torch.bincount(c.table[c.table >= 0].long(), minlength=24).to(torch.int32))
