@@ -528,11 +528,19 @@ int lq_pages_copy(const int32_t *src, const int32_t *dst, const int32_t *count, 
  * accepted[b][0..] names the ones to keep, strictly ascending, ended by a
  * negative entry or by `most`.  Their rows move to the front of the drafts'
  * slots in all layers; new_lens (not lens itself) = lens - n_draft + kept.
- * A row whose list is not ascending or out of range is left as it is. */
+ * A row whose list is not ascending or out of range is left as it is, with
+ * LQ_EF_PAGE.  No row may share a page that another row's drafts move into;
+ * lq_pages_accept_shared sees to that: a row that would have to move a draft
+ * into a page with refs above 1 (drafts that filled a page before a fork) is
+ * left as it is, with LQ_EF_PAGE. */
 int lq_pages_accept(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens, int64_t n_draft,
                     const int32_t *accepted, int64_t most, int32_t *new_lens, int32_t *codes, float *scales,
                     int64_t n_layers, int64_t n_pages, int n_heads, int page_tokens, int head_dim, uint32_t *err,
                     void *stream);
+int lq_pages_accept_shared(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens, const int32_t *refs,
+                           int64_t n_draft, const int32_t *accepted, int64_t most, int32_t *new_lens, int32_t *codes,
+                           float *scales, int64_t n_layers, int64_t n_pages, int n_heads, int page_tokens, int head_dim,
+                           uint32_t *err, void *stream);
 
 /* ------------------------------------------------------------------------
  * Beam search's selection: the n largest of scores[b][k] + ln softmax(x[b][k])[v]

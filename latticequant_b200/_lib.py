@@ -126,6 +126,7 @@ def _declare(lib):
         "lq_pages_compact": ([vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, vp, sz, vp, vp], i32),
         "lq_pages_copy": ([vp, vp, vp, i64, vp, vp, i64, i64, i32, i32, i32, vp, vp], i32),
         "lq_pages_accept": ([vp, i64, i64, vp, i64, vp, i64, vp, vp, vp, i64, i64, i32, i32, i32, vp, vp], i32),
+        "lq_pages_accept_shared": ([vp, i64, i64, vp, vp, i64, vp, i64, vp, vp, vp, i64, i64, i32, i32, i32, vp, vp], i32),
         "lq_beam_select_workspace": ([i32, i64, i64, i64, i64], sz),
         "lq_beam_select": ([vp, i32, i64, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, sz, vp], i32),
         "lq_rans_finish_streams": ([vp, vp, vp, i64, vp, vp, vp], i32),

@@ -275,6 +275,7 @@ __global__ void __launch_bounds__(256) move_pages_kernel(const __grid_constant__
 // ---- accept ------------------------------------------------------------------
 struct AcceptArgs {
     const int32_t *table, *lens, *accepted;
+    const int32_t *refs;  // NULL: every page is its row's own
     int64_t width, n_pages, n_draft, most;
     uint32_t page_log2;
     int32_t *new_lens;
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(128) accept_kernel(const __grid_constant__ Acc
     const int64_t b = blockIdx.x, layer = (int64_t)blockIdx.y * a.n_pages;
     const int32_t *acc = a.accepted + b * a.most;
     const int64_t base = a.lens[b] - a.n_draft;
+    const int32_t *table = a.table + b * a.width;
     __shared__ int s_n;
     if (threadIdx.x < 32) {  // accepted drafts: up to the first negative, strictly ascending
         int n = 0;
@@ -309,6 +311,14 @@ __global__ void __launch_bounds__(128) accept_kernel(const __grid_constant__ Acc
             if (end) break;
         }
         ok = ok && (n == 0 || (base >= 0 && a.lens[b] <= a.width << a.page_log2));
+        if (ok && a.refs) {  // a row that moves moves nothing into a page that somebody else holds too
+            bool shared = false;
+            for (int64_t j = threadIdx.x; j < n; j += 32) {
+                const int32_t p = table[(base + j) >> a.page_log2];
+                shared |= acc[j] != j && p >= 0 && p < a.n_pages && a.refs[p] > 1;
+            }
+            ok = !__any_sync(0xffffffffu, shared);
+        }
         if (threadIdx.x == 0) {
             s_n = ok ? n : 0;
             if (!ok && blockIdx.y == 0) raise_flag(a.err, LQ_EF_PAGE);
@@ -317,7 +327,6 @@ __global__ void __launch_bounds__(128) accept_kernel(const __grid_constant__ Acc
     }
     __syncthreads();
     const int n = s_n;
-    const int32_t *table = a.table + b * a.width;
     const uint32_t mask = (1u << a.page_log2) - 1;
     auto row_of = [&](int64_t tok, int64_t head) -> int64_t {  // -1: no page there
         const int32_t p = table[tok >> a.page_log2];
@@ -484,11 +493,10 @@ extern "C" int lq_pages_copy(const int32_t *src, const int32_t *dst, const int32
     return check_launch();
 }
 
-extern "C" int lq_pages_accept(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens, int64_t n_draft,
-                               const int32_t *accepted, int64_t most, int32_t *new_lens, int32_t *codes, float *scales,
-                               int64_t n_layers, int64_t n_pages, int n_heads, int page_tokens, int head_dim,
-                               uint32_t *err, void *stream) {
-    LQ_NVTX_RANGE();
+static int accept(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens, const int32_t *refs,
+                  int64_t n_draft, const int32_t *accepted, int64_t most, int32_t *new_lens, int32_t *codes,
+                  float *scales, int64_t n_layers, int64_t n_pages, int n_heads, int page_tokens, int head_dim,
+                  uint32_t *err, void *stream) {
     if (!pool_ok(codes, scales, n_layers, n_pages, n_heads, page_tokens, head_dim) || rows < 0 || rows > (1 << 24) ||
         width < 1 || width > (1 << 20) || n_draft < 1 || n_draft > 4096 || most < 0)
         return LQ_ERR_INVALID;
@@ -498,6 +506,7 @@ extern "C" int lq_pages_accept(const int32_t *table, int64_t rows, int64_t width
     a.table = table;
     a.lens = lens;
     a.accepted = accepted;
+    a.refs = refs;
     a.width = width;
     a.n_pages = n_pages;
     a.n_draft = n_draft;
@@ -511,4 +520,24 @@ extern "C" int lq_pages_accept(const int32_t *table, int64_t rows, int64_t width
     a.err = err;
     accept_kernel<<<dim3((unsigned)rows, (unsigned)n_layers), 128, 0, as_stream(stream)>>>(a);
     return check_launch();
+}
+
+extern "C" int lq_pages_accept(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens, int64_t n_draft,
+                               const int32_t *accepted, int64_t most, int32_t *new_lens, int32_t *codes, float *scales,
+                               int64_t n_layers, int64_t n_pages, int n_heads, int page_tokens, int head_dim,
+                               uint32_t *err, void *stream) {
+    LQ_NVTX_RANGE();
+    return accept(table, rows, width, lens, nullptr, n_draft, accepted, most, new_lens, codes, scales, n_layers, n_pages,
+                  n_heads, page_tokens, head_dim, err, stream);
+}
+
+extern "C" int lq_pages_accept_shared(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens,
+                                      const int32_t *refs, int64_t n_draft, const int32_t *accepted, int64_t most,
+                                      int32_t *new_lens, int32_t *codes, float *scales, int64_t n_layers,
+                                      int64_t n_pages, int n_heads, int page_tokens, int head_dim, uint32_t *err,
+                                      void *stream) {
+    LQ_NVTX_RANGE();
+    if (!refs) return LQ_ERR_INVALID;
+    return accept(table, rows, width, lens, refs, n_draft, accepted, most, new_lens, codes, scales, n_layers, n_pages,
+                  n_heads, page_tokens, head_dim, err, stream);
 }

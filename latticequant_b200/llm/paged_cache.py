@@ -86,8 +86,12 @@ class PagedKVCache:
 
     # ---- between steps --------------------------------------------------------
     def accept(self, accepted: torch.Tensor) -> None:
-        """Keep the accepted drafts of the last step (paged.accept_tokens); the rest go."""
-        self.lens = paged.accept_tokens(self.codes, self.scales, self.table, self.lens, self._n_new, accepted, self.err)
+        """Keep the accepted drafts of the last step (paged.accept_tokens); the rest go.
+
+        Accept before a fork: drafts that a fork shared between rows cannot move
+        any more, and a row that would need it is left as it is (flags())."""
+        self.lens = paged.accept_tokens(self.codes, self.scales, self.table, self.lens, self._n_new, accepted, self.err,
+                                        self.refs)
         self.max_len += accepted.shape[1] - self._n_new
         self._slots = None
 

@@ -220,12 +220,17 @@ def copy_pages(codes: torch.Tensor, scales: torch.Tensor, src: torch.Tensor, dst
 
 
 def accept_tokens(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, n_draft: int,
-                  accepted: torch.Tensor, err: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  accepted: torch.Tensor, err: Optional[torch.Tensor] = None,
+                  refs: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Keep the accepted ones of each row's last ``n_draft`` tokens (lq_pages_accept).
 
     accepted int32 (rows, most): draft indices, strictly ascending (a path of
     the tree from its root), padded with -1.  Their rows move to the front of
-    the drafts' slots in all layers.  Returns the new lens."""
+    the drafts' slots in all layers.  Returns the new lens.
+
+    The pages that drafts move into must be their row's own.  A fork after the
+    drafts came in may have shared one; with ``refs`` a row that would move a
+    draft into such a page is left as it is and reported (EF_PAGE)."""
     index, n_pages, H, P, D = _pool(codes, scales, 6)
     if table.dim() != 2 or accepted.dim() != 2:
         raise ValueError("table is (rows, width) and accepted (rows, most)")
@@ -233,6 +238,11 @@ def accept_tokens(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor
     table_p, lens_p = _need(table, _I32, (rows, width), "table", index), _need(lens, _I32, (rows,), "lens", index)
     accepted_p = _need(accepted, _I32, (rows, most), "accepted", index)
     new_lens = torch.empty_like(lens)
-    call("lq_pages_accept", index, table_p, rows, width, lens_p, int(n_draft), accepted_p, most, new_lens.data_ptr(),
-         codes.data_ptr(), scales.data_ptr(), codes.shape[0], n_pages, H, P, D, _ptr(err))
+    rest = (int(n_draft), accepted_p, most, new_lens.data_ptr(), codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+            n_pages, H, P, D, _ptr(err))
+    if refs is None:
+        call("lq_pages_accept", index, table_p, rows, width, lens_p, *rest)
+    else:
+        call("lq_pages_accept_shared", index, table_p, rows, width, lens_p, _need(refs, _I32, (n_pages,), "refs", index),
+             *rest)
     return new_lens

@@ -199,3 +199,46 @@ def test_rollback_behind_a_fork():
         own.append(0, *[torch.cat([x] + [kv[i][b: b + 1] for kv in new], 2) for i, x in enumerate(ctx)])
         assert torch.equal(o[b: b + 1], own.attend(0, q[b: b + 1]))
     assert torch.equal(c.refs, torch.bincount(c.table[c.table >= 0].long(), minlength=24).to(torch.int32))
+
+
+def test_accept_moves_nothing_into_a_shared_page():
+    """A tree of drafts split by a fork: the drafts that filled the page before it are held by both rows."""
+    from latticequant_b200 import _lib
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    ctx, drafts = _kv(g, 1, 14), _kv(g, 1, 5)
+    c = _cache(1, layers=2)
+    c.begin(14)
+    for layer in range(2):
+        c.append(layer, *ctx)
+    c.begin(5)
+    for layer in range(2):
+        c.append(layer, *drafts)
+    c.fork(torch.tensor([0, 0, 0], device="cuda"))
+    codes, scales = c.codes.clone(), c.scales.clone()
+    # row 0 keeps drafts that are in place, row 1 would move draft 3 into slot 15, row 2's list moves only in its own page
+    c.accept(torch.tensor([[0, 1, 2, -1], [0, 3, 4, -1], [0, 1, 2, 4]], dtype=torch.int32, device="cuda"))
+    assert c.flags() == _lib.EF_PAGE
+    assert c.lens.tolist() == [17, 19, 18]
+    own = int(c.table[2, 1])
+    codes[:, own, :, :, 1], scales[:, own, :, :, 1] = codes[:, own, :, :, 2], scales[:, own, :, :, 2]
+    assert torch.equal(c.codes, codes) and torch.equal(c.scales, scales)
+
+
+def test_accept_with_counts_equals_accept_where_nothing_is_shared(P):
+    L, H, page, D, T = 2, 2, 16, 64, 9
+    lens = [T, 40, 33]
+    table = torch.randperm(12, device="cuda").to(torch.int32).view(3, 4)
+    acc = torch.tensor([[0, 2, 5, 8], [1, 3, -1, -1], [0, 1, 2, 3]], dtype=torch.int32, device="cuda")
+    refs = torch.ones(12, dtype=torch.int32, device="cuda")
+    refs[table[1, 0]] = 3  # a shared page in front of the drafts
+    codes = torch.randint(-2**31, 2**31 - 1, (L, 12, 2, H, page, D // 8), dtype=torch.int32, device="cuda")
+    scales = torch.rand(L, 12, 2, H, page, device="cuda")
+    c1, s1, err = codes.clone(), scales.clone(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    a = P.accept_tokens(codes, scales, table, ln, T, acc, err)
+    b = P.accept_tokens(c1, s1, table, ln, T, acc, err, refs)
+    assert a.tolist() == b.tolist() == [4, 33, 28] and int(err.item()) == 0
+    assert torch.equal(codes, c1) and torch.equal(scales, s1)
+    with pytest.raises(ValueError):
+        P.accept_tokens(codes, scales, table, ln, T, acc, err, refs[:3])

@@ -27,3 +27,10 @@ def test_page_operations_refuse_misaligned_workspaces(lib):
                                  None, None) == INVALID
         assert lib.lq_pages_compact(PTR, 8, PTR, PTR, PTR, PTR, PTR, PTR, 1, 8, 1, 16, 64, PTR + off, 1 << 20, None,
                                     None) == INVALID
+
+
+def test_accept_with_counts_refusals(lib):
+    a = [PTR, 2, 4, PTR, PTR, 5, PTR, 3, PTR, PTR, PTR, 1, 8, 1, 16, 64, None, None]
+    for i, v in ((0, None), (2, 0), (3, None), (4, None), (5, 0), (5, 4097), (6, None), (7, -1), (8, None), (14, 15)):
+        assert lib.lq_pages_accept_shared(*a[:i], v, *a[i + 1:]) == INVALID, i
+    assert lib.lq_pages_accept_shared(PTR, 0, *a[2:]) == 0
