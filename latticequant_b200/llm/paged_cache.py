@@ -90,9 +90,12 @@ class PagedKVCache:
 
         Accept before a fork: drafts that a fork shared between rows cannot move
         any more, and a row that would need it is left as it is (flags())."""
+        if self._n_new == 0:
+            raise ValueError("accept takes the drafts of one begin(), once")
         self.lens = paged.accept_tokens(self.codes, self.scales, self.table, self.lens, self._n_new, accepted, self.err,
                                         self.refs)
         self.max_len += accepted.shape[1] - self._n_new
+        self._n_new = 0  # what is left are tokens
         self._slots = None
 
     def fork(self, parents: torch.Tensor, reserve: int = 0) -> None:

@@ -242,3 +242,21 @@ def test_accept_with_counts_equals_accept_where_nothing_is_shared(P):
     assert torch.equal(codes, c1) and torch.equal(scales, s1)
     with pytest.raises(ValueError):
         P.accept_tokens(codes, scales, table, ln, T, acc, err, refs[:3])
+
+
+def test_a_step_is_accepted_once():
+    g = torch.Generator(device="cuda").manual_seed(6)
+    c = _cache(2)
+    with pytest.raises(ValueError):
+        c.accept(torch.zeros(2, 1, dtype=torch.int32, device="cuda"))
+    c.begin(20)
+    c.append(0, *_kv(g, 2, 20))
+    c.begin(3)
+    c.append(0, *_kv(g, 2, 3))
+    keep = torch.tensor([[0, 2], [1, -1]], dtype=torch.int32, device="cuda")
+    c.accept(keep)
+    for between in (lambda: None, lambda: c.fork(torch.tensor([1, 0], device="cuda"))):
+        between()
+        with pytest.raises(ValueError):
+            c.accept(keep)
+    assert c.lens.tolist() == [21, 22] and c.max_len == 22 and c.flags() == 0
