@@ -475,8 +475,9 @@ int lq_paged_append(const void *k, const void *v, int dtype, int64_t n_tokens, i
  *   q        [batch][n_heads * group][n_query][head_dim], LQ_F16 or LQ_BF16,
  *            16-byte aligned, strides (elements) multiples of 8; query head
  *            h * group + g reads KV head h
- *   lens     tokens in the pages, the drafts included; max_len bounds them
- *            (longer ones are cut, with LQ_EF_PAGE)
+ *   lens     tokens in the pages, the drafts included (those past the table's
+ *            table_width pages are cut, with LQ_EF_PAGE); max_len is the length
+ *            that the work is split for: longer rows are right, but slower
  *   mask     bytes [n_query][n_query], sequences mask_stride_b apart (0: one
  *            for all); NULL: causal
  *   out      [batch][n_heads * group][n_query][head_dim] in q's type, aligned

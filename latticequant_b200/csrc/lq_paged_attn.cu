@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(32 * kWarps, 4) paged_attn_kernel(const __grid
     const uint32_t row0 = rt * kTileRows;
     // positions fit 32 bits: a table is at most 2^20 pages of 2^8 tokens
     const int len = (int)paged_len(a, b);
-    const int first = (int)(blockIdx.x * a.chunk), last = (int)min(first + a.chunk, (int64_t)len);
+    const int first = (int)(blockIdx.x * a.chunk), last = paged_split_end(a, first, len);
     const int drafts = len - (int)a.T;  // position of draft 0
     if (len < a.lens[b] && (blockIdx.x | blockIdx.y | threadIdx.x) == 0) raise_flag(a.err, LQ_EF_PAGE);
 
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
     const uint32_t b = bh / a.n_heads, h = bh - b * a.n_heads;
     const float *p = paged_part<D>(a, bh, 0);
     const int64_t step = (int64_t)a.rows * (D + 4);
-    const uint32_t used = (uint32_t)ceil_div(paged_len(a, b), a.chunk);
+    const uint32_t used = min((uint32_t)ceil_div(paged_len(a, b), a.chunk), a.splits);
     float m = kNoRef;
     for (uint32_t s = lane; s < used; s += 32) m = fmaxf(m, p[s * step + (int64_t)a.rows * D + 2 * r]);
 #pragma unroll
@@ -531,10 +531,8 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
     if ((al & 15) != 0 || ((q_stride_b | q_stride_h | q_stride_t) & 7) != 0) return LQ_ERR_INVALID;
     // a lane stores head_dim / 32 elements at once
     if ((reinterpret_cast<uintptr_t>(out) & (head_dim / 16 - 1)) != 0) return LQ_ERR_INVALID;
-    // tokens past max_len would have no split: the caller's bound is the table's at most
     const int64_t cap = table_width * page_tokens;
-    const int64_t bound = max_len < cap ? max_len : cap;
-    const Plan p = plan(batch, n_heads, n_query * group, head_dim, bound);
+    const Plan p = plan(batch, n_heads, n_query * group, head_dim, max_len < cap ? max_len : cap);
     if (const size_t need = workspace_of(p, batch * n_heads * n_query * group, head_dim)) {
         if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return LQ_ERR_INVALID;
         if (workspace_bytes < need) return LQ_ERR_CAPACITY;
@@ -552,7 +550,7 @@ extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b
     a.table_width = table_width;
     a.table_stride = table_stride;
     a.lens = lens;
-    a.bound = bound;
+    a.bound = cap;
     a.mask = mask;
     a.mask_stride_b = mask_stride_b;
     a.n_heads = (uint32_t)n_heads;

@@ -16,7 +16,7 @@ struct PagedAttnArgs {
     const int32_t *table;  // [batch][table_width], rows table_stride apart
     int64_t table_width, table_stride;
     const int32_t *lens;
-    int64_t bound;        // tokens a sequence may have at most
+    int64_t bound;        // tokens that a row of the table holds
     const uint8_t *mask;  // [batch or 1][T][T], or NULL: drafts <= t
     int64_t mask_stride_b;
     uint32_t n_heads, group, T, rows;  // rows = T * group, row = t * group + g
@@ -56,6 +56,11 @@ __device__ __forceinline__ float rcp(float x) {
 
 __device__ __forceinline__ int64_t paged_len(const PagedAttnArgs &a, uint32_t b) {
     return min(max((int64_t)a.lens[b], (int64_t)0), a.bound);
+}
+
+// Where this CTA's split of the tokens ends: the last one takes what lies beyond the length that was planned for.
+__device__ __forceinline__ int paged_split_end(const PagedAttnArgs &a, int first, int len) {
+    return blockIdx.x + 1 < a.splits ? (int)min(first + a.chunk, (int64_t)len) : len;
 }
 
 // Whether position t of sequence b sees draft j.

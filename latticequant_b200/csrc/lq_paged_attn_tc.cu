@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
     const uint32_t b = blockIdx.z, rt = blockIdx.y / a.n_heads, h = blockIdx.y - rt * a.n_heads;
     const uint32_t row0 = rt * COLS;
     const int len = (int)paged_len(a, b);
-    const int first = (int)(blockIdx.x * a.chunk), last = (int)min(first + a.chunk, (int64_t)len);
+    const int first = (int)(blockIdx.x * a.chunk), last = paged_split_end(a, first, len);
     const int drafts = len - (int)a.T;
     if (len < a.lens[b] && (blockIdx.x | blockIdx.y | tid) == 0) raise_flag(a.err, LQ_EF_PAGE);
     const int live = (int)min((uint32_t)COLS, a.rows - row0);

@@ -15,7 +15,9 @@ that the model confirmed; for beams ``fork`` reorders the rows
 layer and has none of these (llm/compressed_kv_cache.py:342-395).
 
 Nothing synchronises with the host: the host keeps an upper bound of the
-lengths (``max_len``), and ``flags()`` reads the error word.
+lengths (``max_len``, which sets how attention splits its work and nothing
+else; a caller that knows better after freeing rows may lower it), and
+``flags()`` reads the error word.
 """
 from __future__ import annotations
 
@@ -42,7 +44,7 @@ class PagedKVCache:
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=dev)
         self.lens = torch.zeros(rows, dtype=torch.int32, device=dev)
         self.err = torch.zeros(1, dtype=torch.int32, device=dev)
-        self.max_len = 0  # no row is longer
+        self.max_len = 0  # no row is longer (but those whose list accept() refused)
         self._n_new = 0
         self._slots: Optional[torch.Tensor] = None
 

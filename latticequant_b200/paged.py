@@ -119,7 +119,7 @@ def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, t
     sees all tokens before them, and draft j where mask[t, j] -- bool (T, T) or
     (B, T, T), e.g. each draft's ancestors and itself -- or, without a mask,
     j <= t.  ``max_len``: an upper bound on ``lens`` known to the host (default:
-    the table's width), which sets the split.  Returns o (B, Hq, T, D) in q's
+    the table's width), which sets the split; longer rows are right, but slower.  Returns o (B, Hq, T, D) in q's
     dtype (and the fp32 (B, Hq, T) log-sum-exp if return_lse); a position that
     sees nothing gives 0 and -inf."""
     index, n_pages, H, P, D = _pool(codes, scales, 5)

@@ -260,3 +260,46 @@ def test_a_step_is_accepted_once():
         with pytest.raises(ValueError):
             c.accept(keep)
     assert c.lens.tolist() == [21, 22] and c.max_len == 22 and c.flags() == 0
+
+
+@pytest.mark.parametrize("T,G,D", [(1, 4, 128), (3, 4, 64), (13, 4, 128), (16, 8, 64)])
+@pytest.mark.parametrize("planned", [0, 1, 130, 700, 2600])
+def test_rows_longer_than_planned_are_read_whole(P, T, G, D, planned):
+    """max_len sets the split; rows beyond it are attended to their end by either kernel, in a cluster or not."""
+    lens = [3000, 131, 40, 2601]
+    codes, scales, table, ln = _filled(P, lens, 2, D, 16)
+    q = torch.randn(4, 2 * G, T, D, device="cuda").to(torch.float16)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want, wl = P.tree_attention(q, codes, scales, table, ln, return_lse=True)
+    o, lse = P.tree_attention(q, codes, scales, table, ln, return_lse=True, max_len=planned, err=err)
+    assert int(err.item()) == 0
+    # two orders of the same sums: fp16's unit roundoff and a weight's, twice
+    top = want.float().abs().amax(-1, keepdim=True)
+    assert bool(((o.float() - want.float()).abs() <= 2e-3 * top + 2 ** -10 * want.float().abs()).all())
+    assert bool(((lse - wl).abs() <= 2e-4 * wl.abs().clamp(min=1)).all())
+
+
+def test_a_refused_row_is_attended_whole():
+    """A list that accept() refuses leaves its row all the drafts, and later steps see them."""
+    from latticequant_b200 import _lib
+
+    g = torch.Generator(device="cuda").manual_seed(7)
+    ctx, drafts, new = _kv(g, 2, 20), _kv(g, 2, 9), _kv(g, 2, 1)
+    q = torch.randn(2, 4, 1, 64, device="cuda", generator=g).to(torch.bfloat16)
+    c = _cache(2)
+    for n, kv in ((20, ctx), (9, drafts)):
+        c.begin(n)
+        c.append(0, *kv)
+    c.accept(torch.tensor([[0], [12]], dtype=torch.int32, device="cuda"))  # 12: no such draft
+    assert c.flags() == _lib.EF_PAGE and c.lens.tolist() == [21, 29]
+    c.err.zero_()
+    c.begin(1)
+    c.append(0, *new)
+    o = c.attend(0, q)
+    assert c.flags() == 0
+    for b, n in ((0, 1), (1, 9)):
+        own = _cache(1)
+        own.begin(20 + n + 1)
+        own.append(0, *[torch.cat([x[b: b + 1], d[b: b + 1, :, :n], y[b: b + 1]], 2) for x, d, y in zip(ctx, drafts, new)])
+        w = own.attend(0, q[b: b + 1])
+        assert bool(((o[b: b + 1] - w).float().abs() <= 2e-3 * w.float().abs().max() + 2 ** -7 * w.float().abs()).all())
