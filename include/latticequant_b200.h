@@ -484,7 +484,8 @@ int lq_paged_append(const void *k, const void *v, int dtype, int64_t n_tokens, i
  *            to head_dim / 16 bytes
  *   lse      optional fp32 [batch][n_heads * group][n_query], natural log.  A
  *            position that sees no token gets o = 0, lse = -inf
- * n_query 1..4096, group 1..64. */
+ * n_query 1..4096, group 1..64.  The workspace (16-byte aligned) that the first
+ * function names is enough for every call with these or fewer tokens. */
 size_t lq_paged_attention_workspace(int64_t batch, int n_heads, int group, int64_t n_query, int head_dim,
                                     int64_t max_len);
 int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,

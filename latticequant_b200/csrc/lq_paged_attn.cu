@@ -460,17 +460,34 @@ struct Plan {
     bool clustered;
 };
 constexpr int64_t kClusterMax = 8, kClusterTokens = 256;  // splits, and the chunk up to which 8 of them are enough
-constexpr int64_t kStartTiles = 3, kShortest = 4, kMostSplits = 512;
+constexpr int64_t kStartTiles = 3, kShortest = 4, kMostSplits = 512, kMostRounds = 16;
+
+// What a plan starts from.
+struct Work {
+    bool few;
+    int tile;
+    int64_t tile_tokens, slots, units, tokens, tiles;  // units: CTAs without a split
+    int64_t most;                                      // splits looked at: past this there are only more starts
+    Work(int64_t batch, int n_heads, int64_t rows, int head_dim, int64_t max_len) {
+        few = rows <= (head_dim == 64 ? 16 : 8);
+        tile = few ? kTileRows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+        tile_tokens = few ? 64 : 128;
+        slots = 148 * (few ? 4 : 1);
+        units = batch * n_heads * ceil_div(rows, tile);
+        tokens = max_len < 1 ? 1 : max_len;
+        tiles = ceil_div(tokens, tile_tokens);
+        most = kMostRounds * slots / units + 1;
+        most = most < kMostSplits ? most : kMostSplits;
+        most = most < tiles ? most : tiles;
+    }
+};
 
 Plan plan(int64_t batch, int n_heads, int64_t rows, int head_dim, int64_t max_len) {
+    const auto [few, tile, tile_tokens, slots, units, tokens, tiles, most] = Work(batch, n_heads, rows, head_dim, max_len);
     Plan p;
-    const bool few = rows <= (head_dim == 64 ? 16 : 8);
-    p.tile = few ? kTileRows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    const int64_t tile_tokens = few ? 64 : 128, slots = 148 * (few ? 4 : 1);
-    const int64_t units = batch * n_heads * ceil_div(rows, p.tile);  // CTAs without a split
-    const int64_t tokens = max_len < 1 ? 1 : max_len, tiles = ceil_div(tokens, tile_tokens);
+    p.tile = tile;
     int64_t best = 0, best_cost = INT64_MAX;
-    for (int64_t s = 1; s <= tiles && s <= kMostSplits; ++s) {
+    for (int64_t s = 1; s <= most; ++s) {
         const int64_t each = ceil_div(tiles, s);
         if (ceil_div(tiles, each) != s) continue;  // no such split
         if (units * s < 2 * slots && each > kShortest && s < kMostSplits && s < tiles) continue;
@@ -479,7 +496,6 @@ Plan plan(int64_t batch, int n_heads, int64_t rows, int head_dim, int64_t max_le
             best_cost = cost;
             best = each;
         }
-        if (units * s > 16 * slots) break;  // only more starts from here
     }
     if (best == 0) best = ceil_div(tiles, kMostSplits);
     p.chunk = best * tile_tokens;
@@ -496,6 +512,14 @@ size_t workspace_of(const Plan &p, int64_t bh_rows, int head_dim) {
     return p.splits > 1 && !p.clustered ? (size_t)bh_rows * p.splits * (head_dim + 4) * 4 : 0;
 }
 
+// What no plan for these or fewer tokens goes beyond.  The splits that plan() takes are not monotone in the length, but
+// the most that it looks at are.
+size_t workspace_bound(int64_t batch, int n_heads, int64_t rows, int head_dim, int64_t max_len) {
+    const Work w(batch, n_heads, rows, head_dim, max_len);
+    const bool clustered = w.few && (w.most <= kClusterMax || w.tokens <= kClusterMax * kClusterTokens);
+    return w.most > 1 && !clustered ? (size_t)(batch * n_heads * rows) * w.most * (head_dim + 4) * 4 : 0;
+}
+
 }  // namespace
 }  // namespace lq
 
@@ -509,8 +533,8 @@ static bool paged_shape_ok(int64_t batch, int n_heads, int group, int64_t n_quer
 
 extern "C" size_t lq_paged_attention_workspace(int64_t batch, int n_heads, int group, int64_t n_query, int head_dim,
                                                int64_t max_len) {
-    if (!paged_shape_ok(batch, n_heads, group, n_query, head_dim) || max_len < 0) return 0;
-    return workspace_of(plan(batch, n_heads, n_query * group, head_dim, max_len), batch * n_heads * n_query * group, head_dim);
+    if (!paged_shape_ok(batch, n_heads, group, n_query, head_dim) || batch == 0 || max_len < 0) return 0;
+    return workspace_bound(batch, n_heads, n_query * group, head_dim, max_len);
 }
 
 extern "C" int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,

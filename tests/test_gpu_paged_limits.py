@@ -303,3 +303,33 @@ def test_a_refused_row_is_attended_whole():
         own.append(0, *[torch.cat([x[b: b + 1], d[b: b + 1, :, :n], y[b: b + 1]], 2) for x, d, y in zip(ctx, drafts, new)])
         w = own.attend(0, q[b: b + 1])
         assert bool(((o[b: b + 1] - w).float().abs() <= 2e-3 * w.float().abs().max() + 2 ** -7 * w.float().abs()).all())
+
+
+@pytest.mark.parametrize("B,H,G,T,D,longest,shorter", [
+    (16, 8, 4, 13, 128, 11328, (11200, 5000, 129)), (32, 8, 4, 1, 128, 2944, (2752, 2100, 64)),
+    (1, 2, 4, 1, 64, 40000, (39000, 20000, 2049)), (2, 2, 7, 9, 64, 9000, (8990, 4097, 640)),
+])
+def test_a_workspace_serves_shorter_bounds_and_narrower_tables(B, H, G, T, D, longest, shorter):
+    """The C entry with the workspace of the longest context, asked for less by max_len and by the table."""
+    from latticequant_b200 import _lib
+
+    lib, page = _lib.lib(), 64
+    need = lib.lq_paged_attention_workspace(B, H, G, T, D, longest)
+    ws = torch.empty(need // 4 + 4, dtype=torch.int32, device="cuda")
+    ws[need // 4:] = 12345
+    codes = torch.full((4, 2, H, page, D // 8), 0x44444444, dtype=torch.int32, device="cuda")
+    scales = torch.ones(4, 2, H, page, device="cuda")
+    width = -(-longest // page)
+    table = torch.randint(0, 4, (B, width), dtype=torch.int32, device="cuda")
+    q = torch.randn(B, H * G, T, D, device="cuda").to(torch.float16)
+    out = torch.empty_like(q)
+    for n in (longest, *shorter):
+        for max_len, cols in ((n, width), (longest, -(-n // page))):
+            lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+            out.fill_(7)
+            status = lib.lq_paged_attention(q.data_ptr(), 1, *q.stride()[:3], codes.data_ptr(), scales.data_ptr(), 4, page,
+                                            table.data_ptr(), cols, width, lens.data_ptr(), max_len, None, 0, B, H, G, T, D,
+                                            1.0, out.data_ptr(), None, ws.data_ptr() if need else None, need, None, None)
+            assert status == 0, (n, max_len, cols)
+            torch.cuda.synchronize()
+            assert not out.any() and (ws[need // 4:] == 12345).all()  # every value is zero

@@ -34,3 +34,14 @@ def test_accept_with_counts_refusals(lib):
     for i, v in ((0, None), (2, 0), (3, None), (4, None), (5, 0), (5, 4097), (6, None), (7, -1), (8, None), (14, 15)):
         assert lib.lq_pages_accept_shared(*a[:i], v, *a[i + 1:]) == INVALID, i
     assert lib.lq_pages_accept_shared(PTR, 0, *a[2:]) == 0
+
+
+@pytest.mark.parametrize("batch,heads,group,n_query,dim", [
+    (16, 8, 4, 13, 128), (32, 8, 4, 1, 128), (1, 8, 4, 1, 128), (1, 1, 1, 1, 64), (4, 4, 7, 64, 128), (8, 4, 8, 31, 64),
+    (3, 2, 5, 3, 64), (1, 4, 7, 2048, 128), (75, 8, 4, 4, 128)])
+def test_attention_workspace_is_enough_for_fewer_tokens(lib, batch, heads, group, n_query, dim):
+    f = lib.lq_paged_attention_workspace
+    lengths = sorted({1, 2, 63, 64, 65, 2048, 2049, 2752, 2944, 11200, 11328, 1 << 20, 1 << 28,
+                      *range(0, 40000, 97)})
+    sizes = [f(batch, heads, group, n_query, dim, n) for n in lengths]
+    assert sizes == sorted(sizes)
