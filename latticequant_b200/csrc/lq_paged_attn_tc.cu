@@ -224,7 +224,8 @@ struct Small {
     alignas(16) float f[X::kSets][X::kN];
     float red[X::kSets][4][X::kN];
     uint32_t bad[X::kStages];  // bit: a page of the stage's tokens lies outside the pool
-    uint32_t tmem, exponent;
+    float back[X::kN];  // what a row's scores are multiplied by where `apart`
+    uint32_t tmem, exponent, apart;
 };
 
 // The lane order of a decoded block: position p holds channel kChannel >> 4p & 15.
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
             init(sm.s_free[i], 4 * X::kGroups);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        sm.exponent = 27;
+        sm.exponent = sm.apart = 0;
     }
     for (int n = tid; n < X::kSets * N; n += kThreads) sm.minus_m[n / N][n % N] = -kNoRef;
 
@@ -330,27 +331,46 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
         // Q: fp16 rows in the decoded blocks' channel order; rows past the last are zero
         float qk = a.qk_log2 * kCodeUnit;
         {
-            if constexpr (BF16) {  // a power of two for all rows puts the largest finite value in [2^10, 2^11)
-                uint32_t e = 27;   // (at least 2^-100)
+            // bf16: a power of two puts the rows' largest finite value in [2^10, 2^11).  Rows down to 2^-kNear of it share
+            // the power, which goes into qk and leaves them every bit; a row further down has its own, and its scores
+            // are multiplied back.
+            if constexpr (BF16) {
+                constexpr uint32_t kLeast = 27, kNear = 10;  // rows under 2^-100 count as 2^-100
+                uint32_t e[kQ], top = kLeast;  // exponent of the chunk's row: the W chunks of a row are neighbouring lanes
     #pragma unroll
                 for (int i = 0; i < kQ; ++i) {
                     const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+                    e[i] = 0;
     #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t lo = w[k] >> 7 & 0xffu, hi = w[k] >> 23 & 0xffu;
-                        e = max(e, max(lo == 0xffu ? 0u : lo, hi == 0xffu ? 0u : hi));
+                        e[i] = max(e[i], max(lo == 0xffu ? 0u : lo, hi == 0xffu ? 0u : hi));
                     }
-                }
-                e = __reduce_max_sync(0xffffffffu, e);
-                if (lane == 0) atomicMax(&sm.exponent, e);
-                sync_softmax<X>();
-                e = sm.exponent;
-                const float f = __uint_as_float((264u - e) << 23);
-                qk *= __uint_as_float((e - 10u) << 23);
     #pragma unroll
-                for (int i = 0; i < kQ; ++i)
+                    for (int o = W / 2; o >= 1; o >>= 1) e[i] = max(e[i], __shfl_xor_sync(0xffffffffu, e[i], o));
+                    top = max(top, e[i]);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) atomicMax(&sm.exponent, top);
+                sync_softmax<X>();
+                top = sm.exponent;
+                qk *= __uint_as_float((top - 10u) << 23);
+    #pragma unroll
+                for (int i = 0; i < kQ; ++i) {
+                    const int at = tid + i * kLoaders;
+                    const uint32_t own = max(e[i], kLeast), down = top - own;
+                    const bool far = e[i] != 0 && down > kNear;
+                    const float f = __uint_as_float((264u - (far ? own : top)) << 23);
                     q[i] = make_uint4(bf16_to_f16(q[i].x, f), bf16_to_f16(q[i].y, f), bf16_to_f16(q[i].z, f),
                                       bf16_to_f16(q[i].w, f));
+                    if (at < kChunks && at % W == 0) {  // 2^-down in two steps: down may reach 227
+                        sm.back[at / W] = far ? __uint_as_float((127u - down / 2) << 23) *
+                                                    __uint_as_float((127u - (down + 1) / 2) << 23)
+                                              : 1.f;
+                        if (far) sm.apart = 1;
+                    }
+                }
+                sync_softmax<X>();
             }
     #pragma unroll
             for (int i = 0; i < kQ; ++i) {
@@ -370,6 +390,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
         float *const minus_m = sm.minus_m[set] + col0, *const f = sm.f[set] + col0;
         float(*const red)[N] = sm.red[set];
         const uint32_t my_p = sp + set * kHalfBytes + tl * 128;
+        const bool apart = BF16 && sm.apart;
         unsigned long long l[C / 2];  // of two columns each, as packed fp32
 #pragma unroll
         for (int c = 0; c < C / 2; ++c) l[c] = 0;
@@ -395,6 +416,10 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, 1)
             float x[C];
             auto scores = [&]() {
                 tmem_load<C>(ts + s * N + my_lanes + col0, x);
+                if (apart) {
+#pragma unroll
+                    for (int c = 0; c < C; ++c) x[c] *= sm.back[col0 + c];
+                }
                 const unsigned long long mul = f2_pack(kx, kx), add = f2_pack(lv, lv);
 #pragma unroll
                 for (int c = 0; c < C; c += 2) f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), mul, add), x[c], x[c + 1]);

@@ -333,3 +333,31 @@ def test_a_workspace_serves_shorter_bounds_and_narrower_tables(B, H, G, T, D, lo
             assert status == 0, (n, max_len, cols)
             torch.cuda.synchronize()
             assert not out.any() and (ws[need // 4:] == 12345).all()  # every value is zero
+
+
+@pytest.mark.parametrize("T,G,D", [(2, 4, 128), (2, 8, 64), (3, 4, 128), (4, 7, 128), (13, 4, 128), (12, 8, 64), (4, 8, 64)])
+def test_query_rows_of_any_magnitude_beside_one_another(P, T, G, D):
+    """bf16 rows 2^60 above, 2^-12, 2^-30 and 2^-90 of their neighbours, zero, and with infinities or NaN: the others'
+    answers are theirs alone.  Bounds as in test_gpu_paged."""
+    import math
+
+    import test_gpu_paged as base
+
+    g = torch.Generator(device="cuda").manual_seed(T * 10 + G)
+    lens = [300, 150]
+    codes, scales, table, ln = base._pool(P, g, lens, 2, D, 16)
+    q = torch.randn(2, 2 * G, T, D, device="cuda", generator=g)
+    q[0, 0, 0] *= 2.0**60
+    q[0, 1, 1] *= 2.0**-12
+    q[1, 0, 0] *= 2.0**-30
+    q[1, 1, 1] *= 2.0**-90
+    q[1, 2, 0] = 0
+    q = q.to(torch.bfloat16)
+    o, lse = P.tree_attention(q, codes, scales, table, ln, return_lse=True)
+    base._check(o, lse, *base._ref(q, codes, scales, table, lens, None, 1 / math.sqrt(D)))
+    bad = q.clone()
+    bad[0, 2, 0, 3], bad[1, 3, 1, 5] = float("inf"), float("nan")
+    o2 = P.tree_attention(bad, codes, scales, table, ln)
+    keep = torch.ones(2, 2 * G, T, dtype=torch.bool, device="cuda")
+    keep[0, 2, 0] = keep[1, 3, 1] = False
+    assert torch.equal(o2[keep], o[keep])
