@@ -60,7 +60,8 @@ __device__ __forceinline__ int64_t paged_len(const PagedAttnArgs &a, uint32_t b)
 
 // Where this CTA's split of the tokens ends: the last one takes what lies beyond the length that was planned for.
 __device__ __forceinline__ int paged_split_end(const PagedAttnArgs &a, int first, int len) {
-    return blockIdx.x + 1 < a.splits ? (int)min(first + a.chunk, (int64_t)len) : len;
+    const int end = first + (int)a.chunk;
+    return end < len && blockIdx.x + 1 < a.splits ? end : len;
 }
 
 // Whether position t of sequence b sees draft j.
