@@ -440,7 +440,8 @@ __global__ void __launch_bounds__(kThreads, 3) beam_part_kernel(const __grid_con
 
 __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const __grid_constant__ BeamArgs a) {
     __shared__ Picker s;
-    __shared__ float lse[kMaxBeams], score[kMaxBeams];
+    // a row's log-sum-exp in two parts: rounded to one, a large maximum would take the digits of the sum
+    __shared__ float top[kMaxBeams], log_sum[kMaxBeams], score[kMaxBeams];
     const int b = blockIdx.x, lane = threadIdx.x & 31;
     after_previous();
     for (int k = threadIdx.x >> 5; k < a.beams; k += kWarps) {
@@ -455,7 +456,8 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const __grid_const
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
-            lse[k] = m + logf(sum);
+            top[k] = m;
+            log_sum[k] = logf(sum);
             score[k] = a.scores[(int64_t)b * a.beams + k];
         }
     }
@@ -465,7 +467,8 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const __grid_const
     auto key_at = [&](int i) {
         const uint64_t lo = keys[i];
         const int k = (int)a.by_keys.div((uint32_t)i);
-        const float v = __fadd_rn(__fsub_rn(from_ordered((uint32_t)(lo >> 24)), lse[k]), score[k]);
+        const float x = from_ordered((uint32_t)(lo >> 24));
+        const float v = __fadd_rn(__fsub_rn(__fsub_rn(x, top[k]), log_sum[k]), score[k]);
         return lo ? Key{ordered(v), (uint64_t)(255 - k) << 56 | lo} : Key{0u, 0ull};
     };
     uint32_t best = 0;

@@ -115,3 +115,31 @@ def test_sums_are_rescaled_when_a_later_tile_is_larger(select):
     got = select(x, s, 6)
     _check(got, x, s, 6)
     assert got[1][3].tolist() == got[1][4].tolist() == got[1][5].tolist() == [-1] * 6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_rows_masked_with_the_types_lowest_value(select, dtype):
+    """All of a row at the lowest finite value is a uniform row; some of it at that value leaves the others' totals alone."""
+    low = torch.finfo(dtype).min
+    x = torch.randn(3, 4, 5000, device="cuda").to(dtype)
+    x[0] = low
+    x[1, :, ::2] = low
+    x[2, 1:] = low
+    s = -torch.rand(3, 4, device="cuda")
+    _check(select(x, s, 10), x, s, 10)
+    got = select(x[:1, :1].contiguous(), torch.zeros(1, 1, device="cuda"), 5)
+    assert got[2].tolist() == [[0, 1, 2, 3, 4]]
+    assert torch.allclose(got[0].double(), torch.full((1, 5), -np.log(5000), dtype=torch.float64, device="cuda"), rtol=2e-6)
+
+
+@pytest.mark.parametrize("offset", [1e3, -3e4, 1e7])
+def test_logits_with_a_large_offset(select, offset):
+    """Steps of 1/4 stay exact up to 2^22; 1e7 leaves whole numbers.  The totals do not depend on the offset."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randint(-30, 30, (2, 3, 9000), device="cuda", generator=g) * (0.25 if abs(offset) < 1e6 else 1.0)
+    s = -4 * torch.rand(2, 3, device="cuda", generator=g)
+    moved = (x + offset).contiguous()
+    assert torch.equal((moved.double() - offset).float(), x)
+    _check(select(moved, s, 12), moved, s, 12)
+    for a, b in zip(select(moved, s, 12), select(x, s, 12)):
+        assert torch.equal(a, b)
