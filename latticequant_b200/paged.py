@@ -75,7 +75,8 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with a contiguous last dimension, 16-byte aligned, its other strides multiples of 8 elements."""
     if t.is_contiguous() and not t.data_ptr() & 15:
-        return t
+        # (a dimension of one element may have any stride)
+        return t.reshape(-1).view(t.shape) if 1 in t.shape and any(s & 7 for s in t.stride()[:-1]) else t
     *outer, last = t.stride()
     if last == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in outer):
         return t

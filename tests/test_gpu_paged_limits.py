@@ -361,3 +361,21 @@ def test_query_rows_of_any_magnitude_beside_one_another(P, T, G, D):
     keep = torch.ones(2, 2 * G, T, dtype=torch.bool, device="cuda")
     keep[0, 2, 0] = keep[1, 3, 1] = False
     assert torch.equal(o2[keep], o[keep])
+
+
+def test_single_tokens_cut_out_of_odd_rows(P):
+    """One token of one head, one position: strides that no element uses may be anything."""
+    codes, scales, table, ln = _filled(P, [50], 1, 128, 16)
+    wide = torch.randn(1, 3 * 128 + 3, device="cuda").to(torch.float16)
+    k, v, q = (wide[:, None, i * 128: (i + 1) * 128] for i in range(3))
+    assert k.stride(0) % 8 and k.is_contiguous()
+    c1, s1 = codes.clone(), scales.clone()
+    slot = torch.tensor([50], device="cuda")
+    a = P.append(codes, scales, k, v, slot, dequantised=True)
+    b = P.append(c1, s1, k.clone().view(-1).view(1, 1, 128), v.clone().view(-1).view(1, 1, 128), slot, dequantised=True)
+    assert torch.equal(codes, c1) and torch.equal(scales, s1) and all(torch.equal(x, y) for x, y in zip(a, b))
+    ln += 1
+    q = q[:, None]
+    assert q.shape == (1, 1, 1, 128) and any(s % 8 for s in q.stride()[:-1])
+    o = P.tree_attention(q, codes, scales, table, ln)
+    assert torch.equal(o, P.tree_attention(q.clone().view(-1).view(1, 1, 1, 128), codes, scales, table, ln))
