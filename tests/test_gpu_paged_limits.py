@@ -379,3 +379,29 @@ def test_single_tokens_cut_out_of_odd_rows(P):
     assert q.shape == (1, 1, 1, 128) and any(s % 8 for s in q.stride()[:-1])
     o = P.tree_attention(q, codes, scales, table, ln)
     assert torch.equal(o, P.tree_attention(q.clone().view(-1).view(1, 1, 1, 128), codes, scales, table, ln))
+
+
+@pytest.mark.parametrize("lens,H,G,T,D,page,dtype,mask", [
+    ([4096], 1, 1, 4096, 64, 64, torch.float16, None),            # a prompt's chunk that is the whole context
+    ([2500, 2048], 1, 3, 2048, 128, 64, torch.bfloat16, None),
+    ([5000, 700, 701], 2, 4, 700, 128, 16, torch.float16, None),  # a chunk after a context
+    ([1900], 1, 2, 700, 128, 256, torch.bfloat16, "tree"),
+    ([3000, 90], 1, 64, 1, 128, 32, torch.float16, None),         # the widest group
+    ([3000, 90], 2, 33, 2, 64, 64, torch.bfloat16, None),
+    ([800, 4], 1, 64, 5, 128, 128, torch.float16, "tree"),
+    ([100, 7], 1, 24, 300, 64, 16, torch.bfloat16, None),         # fewer tokens than positions
+])
+def test_long_chunks_and_wide_groups(P, lens, H, G, T, D, page, dtype, mask):
+    """Bounds as in test_gpu_paged."""
+    import math
+
+    import test_gpu_paged as base
+
+    g = torch.Generator(device="cuda").manual_seed(T + G)
+    codes, scales, table, ln = base._pool(P, g, lens, H, D, page)
+    q = torch.randn(len(lens), H * G, T, D, device="cuda", generator=g).to(dtype)
+    m = base._tree(T, 3, len(lens)) if mask else None
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    o, lse = P.tree_attention(q, codes, scales, table, ln, m, return_lse=True, err=err)
+    assert int(err.item()) == 0
+    base._check(o, lse, *base._ref_gpu(q, codes, scales, table, ln, m, 1 / math.sqrt(D)))
