@@ -17,6 +17,9 @@
 
 namespace lq {
 
+// The word of a block of zeros (u = 8 throughout).  A vector of them has scale 1.
+constexpr uint32_t kZeroWord = 0x44444444u;
+
 __host__ __device__ constexpr bool paged_page_ok(int p) { return p >= 16 && p <= 256 && (p & (p - 1)) == 0; }
 __host__ __device__ constexpr bool paged_dim_ok(int d) { return d == 64 || d == 128; }
 

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
     // a vector with a NaN or an infinity is stored as zeros and reported
     const bool zero = !finite || amax < 1e-6f;
     const float s = zero ? 1.0f : __fmul_rn(amax, kInvBound);
-    uint32_t word = 0x44444444u;  // the zero point: u = 8 in bits 27..30, 23..26, .., u7 >> 1 = 4
+    uint32_t word = kZeroWord;  // u = 8 in bits 27..30, 23..26, .., u7 >> 1 = 4
     float q[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (!zero) {
         float y[8];

@@ -282,6 +282,24 @@ __global__ void __launch_bounds__(32 * kWarps, 4) paged_attn_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < 2; ++c) grow |= fmaxf(s[c], s[2 + c]) > m[c] + kRefSlack;
         if (__any_sync(0xffffffffu, grow)) {
+            // V vectors of zeros move no reference.  A lane holds blocks of four tokens, and the lanes of its t their others.
+            uint32_t zero[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bool z = true;
+#pragma unroll
+                for (int j = 0; j < VW; ++j) z = z && x.v[i][j] == kZeroWord;
+                zero[i] = __ballot_sync(0xffffffffu, z);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {  // token g + 8r is the (g & 1)-th of half r for the lanes with t = g / 2
+                const uint32_t all = (g & 1 ? zero[2 * r + 1] : zero[2 * r]) >> (g >> 1) & 0x11111111u;
+                if (all == 0x11111111u) {
+                    rvs[r] *= kZeroInv;
+                    s[2 * r] += kZeroLog2;
+                    s[2 * r + 1] += kZeroLog2;
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float mx = fmaxf(s[c], s[2 + c]);

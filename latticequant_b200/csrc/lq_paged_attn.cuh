@@ -37,6 +37,12 @@ struct PagedAttnArgs {
 // the 2^11 left let the maximum grow before M has to move again.
 constexpr float kNoRef = -1e30f, kRefSlack = 15.f, kRefBelow = 4.f;
 
+// A V vector of zeros is stored with scale 1, and where it holds most of the
+// weight that scale would move M so far up that the others' weights leave
+// fp16's range.  Its product with the point is zero whatever the scale is, so
+// one that is about to move M counts as 2^-60 instead.
+constexpr float kZeroLog2 = -60.f, kZeroInv = 0x1p60f;
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -405,3 +405,32 @@ def test_long_chunks_and_wide_groups(P, lens, H, G, T, D, page, dtype, mask):
     o, lse = P.tree_attention(q, codes, scales, table, ln, m, return_lse=True, err=err)
     assert int(err.item()) == 0
     base._check(o, lse, *base._ref_gpu(q, codes, scales, table, ln, m, 1 / math.sqrt(D)))
+
+
+@pytest.mark.parametrize("T,D", [(1, 64), (1, 128), (3, 64), (4, 128), (12, 64), (24, 128)])
+@pytest.mark.parametrize("vmag,boost", [(1.0, 18), (0.03, 14), (0.03, 18), (1e-3, 10), (1e-3, 18)])
+def test_a_zero_value_that_holds_most_of_the_weight(P, T, D, vmag, boost):
+    """A sink: its V is zero (stored with scale 1) and its score `boost` above the rest; what the others leave in the
+    output keeps its digits.  Bounds as in test_gpu_paged."""
+    import math
+
+    import test_gpu_paged as base
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n = 400
+    kv = torch.randn(2, n, 1, D, device="cuda", generator=g)
+    kv[1] *= vmag
+    u = torch.randn(D, device="cuda", generator=g)
+    u /= u.norm()
+    kv[0] -= (kv[0] @ u)[..., None] * u
+    for at in (7, 200):  # two of them, the second 2 below the first
+        kv[0, at, 0], kv[1, at] = u * (boost - (at > 7) * 2) * math.sqrt(D) / 8, 0
+    kv[1, 300] = 0  # and an ordinary one
+    q = torch.randn(1, 4, T, D, device="cuda", generator=g)
+    q = (q - (q @ u)[..., None] * u + 8 * u).to(torch.bfloat16)
+    codes, scales, _ = P.empty_pool(1, 8, 1, D, 64)
+    P.append(codes[0], scales[0], kv[0].to(torch.bfloat16), kv[1].to(torch.bfloat16), torch.arange(n, device="cuda"))
+    table = torch.arange(8, device="cuda", dtype=torch.int32)[None].contiguous()
+    ln = torch.tensor([n], dtype=torch.int32, device="cuda")
+    o, lse = P.tree_attention(q, codes[0], scales[0], table, ln, return_lse=True)
+    base._check(o, lse, *base._ref(q, codes[0], scales[0], table, [n], None, 1 / math.sqrt(D)))
