@@ -74,12 +74,11 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with a contiguous last dimension, 16-byte aligned, its other strides multiples of 8 elements."""
-    if t.is_contiguous() and not t.data_ptr() & 15:
-        # (a dimension of one element may have any stride)
-        return t.reshape(-1).view(t.shape) if 1 in t.shape and any(s & 7 for s in t.stride()[:-1]) else t
-    *outer, last = t.stride()
-    if last == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in outer):
+    s = t.stride()  # of three or four dimensions
+    if s[-1] == 1 and not (t.data_ptr() & 15 or (s[0] | s[1] | s[-2]) & 7):
         return t
+    if t.is_contiguous() and not t.data_ptr() & 15:  # (a dimension of one element may have any stride)
+        return t.reshape(-1).view(t.shape)
     return t.clone(memory_format=torch.contiguous_format)
 
 
