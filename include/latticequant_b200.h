@@ -502,7 +502,7 @@ int lq_paged_attention(const void *q, int q_dtype, int64_t q_stride_b, int64_t q
  * refs is 1; other children, and every child of a row whose page somebody else
  * names too, get fresh pages, the lowest free ones in order of child and
  * column, with the live rows copied in all layers.  Entries past the reserve
- * are -1.  Out of place: outputs alias no input.  Too few free pages leave
+ * are -1.  The workspace is 4-byte aligned.  Out of place: outputs alias no input.  Too few free pages leave
  * -1 entries and raise LQ_EF_CAPACITY. */
 size_t lq_pages_fork_workspace(int64_t rows, int64_t children, int64_t n_pages);
 int lq_pages_fork(const int32_t *table, int64_t rows, int64_t width, const int32_t *lens, const int32_t *refs,
@@ -513,7 +513,8 @@ int lq_pages_fork(const int32_t *table, int64_t rows, int64_t width, const int32
 /* Move the live pages to the front of the pool: with n_live pages in use, those
  * at or above n_live go, in order, to the free ones below it, in all layers.
  *   table    [entries] old pages (any number of rows), new_table the new ones
- *   n_live   one int32 on the device.  Outputs alias no input. */
+ *   n_live   one int32 on the device.  Outputs alias no input; the workspace
+ *            is 4-byte aligned. */
 size_t lq_pages_compact_workspace(int64_t n_pages);
 int lq_pages_compact(const int32_t *table, int64_t entries, const int32_t *refs, int32_t *new_table,
                      int32_t *new_refs, int32_t *n_live, int32_t *codes, float *scales, int64_t n_layers,

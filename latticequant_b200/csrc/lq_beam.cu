@@ -1,7 +1,8 @@
 // lq_beam.cu -- beam search's selection over beams and vocabulary.
 //
 // For every sequence with beams k and words v:
-//   lp[k][v] = x[k][v] - ln sum_v exp(x[k][v]),   total = scores[k] + lp
+//   lp[k][v] = (x[k][v] - m[k]) - ln sum_v exp(x[k][v] - m[k]),   m[k] = max_v x[k][v]
+//   total = scores[k] + lp
 // the n largest totals, best first; equal totals go to the lower beam, then
 // the larger logit, then the lower word.  A candidate needs a total above
 // -inf (a banned word, a NaN logit or a dead beam gives none); places left
@@ -24,10 +25,10 @@
 //       reach it are ranked by counting.
 //   beam_merge_kernel  a CTA per sequence joins the parts' statistics and
 //       picks the n best totals the same way.
-// 32 sequences of 8 beams over 128,256 words in bf16 take 27.5 us (2.4 TB/s):
+// 32 sequences of 8 beams over 128,256 words in bf16 take 27.2 us (2.4 TB/s):
 // 256 rows give 148 SMs 1.7 CTAs each, and more parts a row (29 us with two, 32
 // with four) cost more in their starts and rankings than they even out.
-// 4 beams over 32,000 words take 8.6 us, most of it the two launches' latency.
+// 4 beams over 32,000 words take 8.6-9.1 us, most of it the two launches' latency.
 // A part with so many equal logits that a list or the ranking overflows is ranked by
 // n rounds of a block-wide maximum instead, over the logits in memory.
 #include "lq_attn_common.cuh"

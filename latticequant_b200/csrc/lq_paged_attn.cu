@@ -24,11 +24,11 @@
 // tokens; V's A registers pair two tokens' decoded channels by byte permutes.
 //
 // Registers feed the MMAs, no shared memory: with 8 rows a tile's MMAs are few,
-// and what bounds the kernel is issue, most of it the decode (488 instructions a
-// warp and tile of 16 tokens; 70% of issue slots, the integer ALU over half).  The next tile's words load into the registers
-// that this tile's were decoded from.  32 sequences of 16,384 tokens, 8 KV
-// heads of 128, 4 query heads each: 194-198 us, 2.9 TB/s; 1 sequence of 777
-// tokens: 6.0 us.
+// and what bounds the kernel is issue, most of it the decode (489 instructions a
+// warp and tile of 16 tokens; 66% of issue slots, the integer ALU over half).
+// The next tile's words load into the registers that this tile's were decoded
+// from.  32 sequences of 16,384 tokens, 8 KV heads of 128, 4 query heads each:
+// 195 us, 2.9 TB/s; 1 sequence of 777 tokens: 6.3 us.
 #include "lq_paged.cuh"
 #include "lq_paged_attn.cuh"
 
@@ -455,10 +455,11 @@ int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st
 //
 // Few rows go to the kernel of this file, the others to tcgen05.  A row tile
 // takes the decode again, so 16 rows of 128 channels are slower here (us, this
-// kernel : tcgen05; 8 KV heads): 377 : 278 for 32 x 16,384 tokens and 25 : 22 for 8 x
-// 2,048, where 8 rows are 197 : 247 for the first.  64 channels give a tile half the
-// decode: 16 rows 243 : 243 (32 x 16,384), 38.8 : 46.0 (8 x 8,192) and 9.5 : 12.0
-// (4 x 2,048), but 24 rows 341 : 269, 50.4 : 51.7 and 15.4 : 14.3.
+// kernel : tcgen05; 8 KV heads): 379 : 245 for 32 x 16,384 tokens and 25 : 22 for 8 x
+// 2,048, where 8 rows are 197 : 241 for the first.  64 channels give a tile half the
+// decode: 16 rows 244 : 296 (32 x 16,384), 39.1 : 56.6 (8 x 8,192) and 9.9 : 14.7
+// (4 x 2,048); against a form of 16 columns, no longer here, 243 : 243, 38.8 : 46.0
+// and 9.5 : 12.0.  24 rows are 340 : 250, 50.3 : 50.4 and 15.8 : 14.8.
 //
 // The CTAs of a call come in rounds of as many as the GPU holds, so the number
 // of splits is the one whose rounds times a CTA's time (its tiles, and
@@ -466,8 +467,8 @@ int launch_dim(const PagedAttnArgs &a, int tile, uint32_t batch, cudaStream_t st
 // two rounds where the tokens allow chunks of kShortest tiles, for lengths that
 // differ from the bound.  (Tree of 13 over
 // 16 sequences of up to 8,190 tokens, mean over eight draws of their lengths:
-// no such floor 95.8 us, one round 81.2, two 80.7, three 81.3, five 93.9; tree
-// of 64 over 4 x 32,768 tokens: 5 splits 308 us, 6 326, 4 371.)
+// no such floor 92.7 us, one round 83.1, two 75.2, three 74.9, five 83.4; tree
+// of 64 over 4 x 32,768 tokens: 5 splits 303 us, 6 318, 4 365.)
 // Up to kClusterMax splits of the few-rows kernel form a cluster and join over
 // its shared memory, which spares the second launch and the workspace; short
 // contexts take fewer splits for it than would fill the GPU.

@@ -25,15 +25,16 @@
 // decoders do.
 //
 // 64 positions over 4 sequences of 32,768 tokens (448 rows of 4 KV heads of 128):
-// 308 us, 390 TFLOP/s, bound by issue: 7,290 instructions and 2,940 cycles a tile
-// of 128 tokens and 64 rows.  Earlier forms of the product took 749 us (mma.sync
+// 303 us, 397 TFLOP/s, bound by issue (69% of the slots): 7,220 instructions and
+// 2,630 cycles a tile of 128 tokens and 64 rows.  Earlier forms of the product took 749 us (mma.sync
 // from registers) and 413 (tcgen05 with one barrier-synchronised part).
 //
 // M is a reference per row, moved only when an x exceeds it by kRefSlack,
 // which a vote of the 128 threads finds; O is then rescaled in TMEM.
 //
 // Every wait is bounded (LQ_EF_TIMEOUT after about a second; the results are
-// then wrong, and the thread's later waits return at once).
+// then wrong, the thread's later waits return at once, and nothing more is
+// started).
 #include "lq_paged_attn.cuh"
 
 namespace lq {

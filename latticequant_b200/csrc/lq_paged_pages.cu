@@ -11,11 +11,12 @@
 // input still owns and write pages that its input had free, so nothing is
 // overwritten that a later copy reads, and no order between copies matters.
 // Data moves at 16 bytes a thread.  Compacting 512 pages, half of them live, in
-// 16 layers (285 MB) takes 47.5 us, 6.0 TB/s; forking 32 beams in 32 layers (23
-// MB) 11 us (one by one under a profiler, from cold caches, the plan takes 7.8 and
-// the copies 12.1); accepting 5 drafts of 32 rows in
-// 32 layers 7 us.  The plans are one CTA each because they are prefix sums over
-// a few thousand counts, shorter than a launch.
+// 16 layers (285 MB) takes 47.5-52 us, 5.5-6.0 TB/s; forking 32 beams in 32 layers
+// (23 MB) 11.5 us; accepting 5 drafts of 32 rows in 32 layers 7.1 us.  The plans
+// are one CTA each, prefix sums over the pool's counts.  A plan's time grows with
+// the pool: reserving a token for 32 rows takes 5.3 us with 632 pages, 6.9 with
+// 8,192 and 12.3 with 32,768; forking them with the free pages at the end of the
+// pool 10.4, 15.9 and 31.3.
 #include "lq_paged.cuh"
 
 namespace lq {

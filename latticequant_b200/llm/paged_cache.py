@@ -54,7 +54,11 @@ class PagedKVCache:
 
     # ---- a step -------------------------------------------------------------
     def begin(self, n: int) -> None:
-        """Make room for n tokens a row and count them in."""
+        """Make room for n tokens a row and count them in.
+
+        Rows of different lengths (prompts) take the longest's n, and accept()
+        then keeps each row's own tokens, 0, 1, ... with -1 for the padding.
+        Attention and accept() take up to 4,096 tokens a row."""
         self.fork(torch.arange(self.rows, device=self.table.device), reserve=n)
         self.lens = self.lens + n
         self.max_len += n

@@ -434,3 +434,26 @@ def test_a_zero_value_that_holds_most_of_the_weight(P, T, D, vmag, boost):
     ln = torch.tensor([n], dtype=torch.int32, device="cuda")
     o, lse = P.tree_attention(q, codes[0], scales[0], table, ln, return_lse=True)
     base._check(o, lse, *base._ref(q, codes[0], scales[0], table, [n], None, 1 / math.sqrt(D)))
+
+
+def test_prompts_of_different_lengths_padded_to_one():
+    """begin() with the longest, accept() with each row's own tokens: the rows are those of caches of their own."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    lens, n = [37, 3, 0, 20], 37
+    ctx, new = _kv(g, 4, n), _kv(g, 4, 1)
+    q = torch.randn(4, 4, 1, 64, device="cuda", generator=g).to(torch.bfloat16)
+    c = _cache(4)
+    c.begin(n)
+    c.append(0, *ctx)
+    at = torch.arange(n, device="cuda", dtype=torch.int32)[None]
+    c.accept(torch.where(at < torch.tensor(lens, device="cuda")[:, None], at, -1).to(torch.int32))
+    assert c.lens.tolist() == lens and c.max_len == n
+    c.begin(1)
+    c.append(0, *new)
+    o = c.attend(0, q)
+    for b, m in enumerate(lens):
+        own = _cache(1)
+        own.begin(m + 1)
+        own.append(0, *[torch.cat([x[b: b + 1, :, :m], y[b: b + 1]], 2) for x, y in zip(ctx, new)])
+        assert torch.equal(o[b: b + 1], own.attend(0, q[b: b + 1]))
+    assert c.flags() == 0
