@@ -20,7 +20,10 @@
 // so the fp16 weights w stay within 2^15 whatever the scales are.  M is a
 // reference, not the running maximum: it moves (to the maximum less 4) only
 // when an x exceeds it by 15, which a warp vote finds; the statistics are then
-// rescaled.  W^T reaches its B registers with one 8x8 transpose per 8
+// rescaled.  (x is one fp32 number: beyond scores of about 1e4 its rounding
+// reaches that of the fp16 weights, and beyond 1e7 log2(vs) is lost in it, which
+// shows where keys are equal; a row whose scores all lie under -1e30 counts as
+// seeing nothing.)  W^T reaches its B registers with one 8x8 transpose per 8
 // tokens; V's A registers pair two tokens' decoded channels by byte permutes.
 //
 // Registers feed the MMAs, no shared memory: with 8 rows a tile's MMAs are few,
